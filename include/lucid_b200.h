@@ -459,6 +459,77 @@ int lq_groupwise_matmul(const void* x, int x_dtype, size_t M, size_t ldx, const 
                         const float* scales, const float* biases, size_t N, size_t K, int group_size,
                         int bits, const float* bias, int relu, void* out, size_t ldo, void* stream);
 
+/* ---- microscaled 4-bit floating point (MXFP4) ------------------------------------------- */
+
+/* A block of 32 consecutive values of a row holds 4-bit floats (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives) and shares a power-of-two scale kept as its biased exponent (E8M0; 255 = NaN).
+ * scale = 2^max(floor(log2 amax) - 2, -127) (a block of zeros: byte 0); an element is x / scale rounded
+ * to the nearest element, ties to the even mantissa, clamped at 6.  A block that holds a NaN or an
+ * infinity takes byte 255 and zero codes: it decodes to NaN.  No counterpart in the reference, whose
+ * 4-bit route is the integer one below; the format is the OCP Microscaling one.
+ *   codes:  (rows, K / 2) bytes, value 2i in the low half of byte i.
+ *   scales: lq_mx_scale_bytes(rows, K) bytes, tiles of 128 rows x 8 blocks,
+ *           tile (row / 128, block / 8) of ceil(K / 256) tiles a row, inside it byte
+ *           (block % 8 / 4) * 512 + (row % 32) * 16 + (row % 128 / 32) * 4 + block % 4.
+ * K is a multiple of 32; x, codes, scales and out are 16-byte aligned.  Empty matrices are no-ops. */
+size_t lq_mx_scale_bytes(size_t rows, size_t K);
+/* x: (rows, K), LQ_F32 | LQ_BF16, row stride ldx elements (16-byte aligned rows).  The padding of the
+ * scale tiles is written as 0. */
+int lq_mx_quantize(const void* x, int in_dtype, size_t rows, size_t K, size_t ldx, uint8_t* codes,
+                   uint8_t* scales, void* stream);
+/* out: (rows, K) contiguous, LQ_F32 | LQ_BF16 (both hold every finite value of the format exactly). */
+int lq_mx_dequantize(const uint8_t* codes, const uint8_t* scales, size_t rows, size_t K, void* out,
+                     int out_dtype, void* stream);
+/* out = decode(encode(x)) over n contiguous values (n a multiple of 32), out of x's dtype.  mask
+ * (optional, n / 8 bytes): bit i of byte j is set where value 8j + i was rounded inside the grid
+ * (|x| / scale < 7), the values whose gradient passes straight through. */
+int lq_mx_fake_quantize(const void* x, int dtype, size_t n, void* out, uint8_t* mask, void* stream);
+/* out = grad where the mask bit is set, 0 elsewhere. */
+int lq_mx_fake_quantize_grad(const void* grad, int dtype, const uint8_t* mask, size_t n, void* out,
+                             void* stream);
+/* out (M, N) = a (M, K) * w (N, K)^T (+ bias[N], float32) (ReLU), float32 accumulation; out LQ_F32 |
+ * LQ_BF16, row stride ldo elements.  status: as for lq_gemm_s8. */
+int lq_mx_matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes,
+                 const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
+                 int out_dtype, size_t ldo, int32_t* status, void* stream);
+/* lq_mx_quantize of x into the workspace, then lq_mx_matmul. */
+size_t lq_mx_linear_workspace_bytes(size_t M, size_t K);
+int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_t* w_codes,
+                 const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
+                 int out_dtype, size_t ldo, uint8_t* workspace, size_t workspace_bytes, int32_t* status,
+                 void* stream);
+
+/* ---- quantized key / value cache -------------------------------------------------------- */
+
+/* A cache of n_pages pages of `page` tokens; slot s = page index * page + offset.  codes and scales of
+ * keys and of values, each (slots, heads, ..) contiguous and 16-byte aligned:
+ *   LQ_KV_INT8:  int8 codes (.., dim), float32 scales (slots, heads); the arithmetic of
+ *                lq_quantize_per_token on the grid [-128, 127] with eps 1e-8, a (token, head) being a row;
+ *                a row that holds a NaN or an infinity takes a NaN scale.  dim % 16 == 0.
+ *   LQ_KV_MXFP4: codes (.., dim / 2) and scale bytes (.., dim / 32) in block order.  dim % 32 == 0.
+ * dim <= 1024.  No counterpart in the reference. */
+enum lq_kv_format { LQ_KV_INT8 = 0, LQ_KV_MXFP4 = 1 };
+
+/* Encode k and v, (tokens, heads, dim) with element strides (token, head) and contiguous dim, LQ_F32 |
+ * LQ_BF16, into slots[0..tokens) (int32 or int64: slot_bits).  A negative slot is skipped (padding); a
+ * slot >= n_slots is skipped and writes LQ_ERR_SHAPE to *status (optional).  A slot that occurs more
+ * than once keeps the last of its tokens. */
+int lq_kv_write(const void* k, const void* v, int in_dtype, size_t tokens, size_t heads, size_t dim, size_t k_token,
+                size_t k_head, size_t v_token, size_t v_head, const void* slots, int slot_bits, size_t n_slots,
+                int format, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t* status,
+                void* stream);
+/* Decode `total` packed rows: row r with cu_seqlens[b] <= r < cu_seqlens[b + 1] (int32, seqs + 1 entries,
+ * ascending) is position starts[b] (NULL: 0) + r - cu_seqlens[b] of sequence b, held in page
+ * table[b * table_stride + position / page].  A position past the table's max_blocks columns or a page
+ * outside the cache reads as zeros and writes LQ_ERR_SHAPE to *status (optional).  Rows outside
+ * [cu_seqlens[0], cu_seqlens[seqs]) are left as they are, or zeroed when clear_tail != 0.  out_k / out_v:
+ * LQ_F32 | LQ_BF16, element strides (token, head), contiguous dim, 16-byte aligned rows. */
+int lq_kv_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int format,
+               size_t n_pages, size_t page, size_t heads, size_t dim, const int32_t* table, size_t table_stride,
+               size_t max_blocks, const int32_t* cu_seqlens, const int32_t* starts, size_t seqs, size_t total,
+               void* out_k, void* out_v, int out_dtype, size_t k_token, size_t k_head, size_t v_token, size_t v_head,
+               int clear_tail, int32_t* status, void* stream);
+
 /* ---- quantized embedding tables -------------------------------------------------------- */
 
 /* Gather + dequantize of the rows of a per-row int8 table.  Replaces the forward of

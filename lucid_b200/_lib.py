@@ -24,6 +24,7 @@ F32, BF16, S8, U8, S16, S32 = 0, 1, 2, 3, 4, 5
 PER_TENSOR, PER_ROW, PER_COL = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_SILU_GATE = 0, 1, 2
 MERGE_ADD, MERGE_MUL, MERGE_ADD_RELU, MERGE_COPY = 0, 1, 2, 3
+KV_INT8, KV_MXFP4 = 0, 1
 ERR_TIMEOUT = 8
 
 _TORCH_CODE = {
@@ -140,6 +141,23 @@ _SIGNATURES = {
     "lq_groupwise_matmul": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
                                       C.c_void_p, C.c_size_t, C.c_size_t, C.c_int, C.c_int, C.c_void_p, C.c_int,
                                       C.c_void_p, C.c_size_t, C.c_void_p]),
+    "lq_mx_scale_bytes": (C.c_size_t, [C.c_size_t, C.c_size_t]),
+    "lq_mx_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                 C.c_void_p]),
+    "lq_mx_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p]),
+    "lq_mx_fake_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "lq_mx_fake_quantize_grad": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "lq_mx_matmul": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t,
+                               C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "lq_mx_linear_workspace_bytes": (C.c_size_t, [C.c_size_t, C.c_size_t]),
+    "lq_mx_linear": (C.c_int, [C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t,
+                               C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p,
+                               C.c_size_t, C.c_void_p, C.c_void_p]),
+    "lq_kv_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int] + [C.c_size_t] * 7 +
+                    [C.c_void_p, C.c_int, C.c_size_t, C.c_int] + [C.c_void_p] * 6),
+    "lq_kv_read": (C.c_int, [C.c_void_p] * 4 + [C.c_int] + [C.c_size_t] * 4 + [C.c_void_p, C.c_size_t, C.c_size_t] +
+                   [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int] +
+                   [C.c_size_t] * 4 + [C.c_int, C.c_void_p, C.c_void_p]),
     "lq_embedding_s8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_int,
                                   C.c_size_t, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_longlong, C.c_void_p,
                                   C.c_int, C.c_void_p, C.c_void_p]),
@@ -236,6 +254,17 @@ def ptr(t):
 
 def stream_ptr(device=None):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def call(name: str, device: torch.device, *args) -> None:
+    """One library call on ``device`` and its current stream (which is the entry's last argument),
+    its status checked."""
+    fn = getattr(load(), name)
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
 
 
 # per-(device, stream) zero-initialised workspace for the per-tensor range reduction

@@ -8,6 +8,8 @@ package's streaming kernels around a library float GEMM.  ``"mlx_group"`` keeps
 the reference's meaning too: ``convert`` / ``quantize_dynamic`` route the Linear
 family to the weight-only group-wise layer (``QuantizedLinearMLX``, here on this
 library's CUDA kernels), everything else takes the dequantize-to-float route.
+``"mxfp4"`` (also of this build) routes the Linear family to microscaled 4-bit floats
+(``MXLinear``; under ``prepare_qat`` to its training form), everything else as ``"reference"``.
 Unlike the reference, ``"auto"`` does not pick that route: it selects the integer
 W8A8 path.
 """
@@ -16,7 +18,7 @@ from __future__ import annotations
 
 from . import _lib
 
-_VALID = ("auto", "b200_i8", "mlx_group", "reference")
+_VALID = ("auto", "b200_i8", "mlx_group", "mxfp4", "reference")
 
 
 class _QuantizedBackend:
@@ -35,7 +37,7 @@ class _QuantizedBackend:
     def engine(self, value: str) -> None:
         if value not in _VALID:
             raise ValueError(
-                "quantized.engine must be 'auto'/'b200_i8'/'mlx_group'/'reference', "
+                "quantized.engine must be 'auto'/'b200_i8'/'mlx_group'/'mxfp4'/'reference', "
                 f"got {value!r}")
         self._engine = value
 
@@ -47,6 +49,11 @@ class _QuantizedBackend:
         """Whether ``convert`` / ``quantize_dynamic`` route Linear layers to the group-wise
         weight-only kernel (lucid/backends/__init__.py:90-96)."""
         return self._engine == "mlx_group"
+
+    def use_mx(self) -> bool:
+        """Whether ``convert`` / ``quantize_dynamic`` / ``prepare_qat`` route Linear layers to
+        microscaled 4-bit floats."""
+        return self._engine == "mxfp4"
 
 
 quantized = _QuantizedBackend()

@@ -16,10 +16,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 SOURCES = ["capi.cu", "stream_kernels.cu", "histogram.cu", "embedding.cu", "exchange.cu", "lstm.cu", "groupwise.cu",
-           "gemm_s8.cu"]
+           "gemm_s8.cu", "microscale.cu", "gemm_mx.cu", "kvcache.cu"]
 # the test-only library: the GEMM with its wait-expiry hook compiled in (-DLQ_TESTING)
 TEST_SOURCES = ["capi.cu", "gemm_s8.cu"]
-HEADERS = ["common.cuh", os.path.join(ROOT, "include", "lucid_b200.h")]
+HEADERS = ["common.cuh", "microscale.cuh", os.path.join(ROOT, "include", "lucid_b200.h")]
 LIB = os.path.join(HERE, "liblucid_b200.so")
 TEST_LIB = os.path.join(HERE, "liblucid_b200_testing.so")
 

@@ -1,0 +1,323 @@
+// The quantized key / value cache: rows encoded as they are written, and read back by page table.
+//
+// A cache row is one token's (heads, dim) values, kept contiguous (page, offset, head, dim), so a write is one
+// pass over the new tokens and a read one pass over the tokens asked for; both are bound by HBM.  Two formats:
+// int8 codes with one float32 scale per (token, head) -- the arithmetic of the per-token encode -- and
+// MXFP4 along the head dimension.
+#include <cuda_fp16.h>
+
+#include "microscale.cuh"
+
+namespace lq {
+namespace {
+
+using mx::Chunk;
+using bf16 = __nv_bfloat16;
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = 1024;
+
+struct Side {          // keys or values
+  const void* x;       // new rows (write) / unused
+  long long x_token, x_head;
+  uint8_t* codes;
+  uint8_t* scales;     // float32 (int8 format) or scale bytes
+  void* out;           // read: destination
+  long long out_token, out_head;
+};
+
+__device__ __forceinline__ long long index_at(const void* p, int bits, size_t i) {
+  return bits == 64 ? __ldg(reinterpret_cast<const long long*>(p) + i) : (long long)__ldg(reinterpret_cast<const int*>(p) + i);
+}
+
+// ---- write ---------------------------------------------------------------------------------------------
+
+// When a slot occurs more than once in a call, the last of its tokens is the one that is kept: each CTA
+// enters its tokens' slots into a hash table in shared memory (the latest token of a slot wins there) and
+// looks the slots of all later tokens up in it.  The rule needs no state between launches and its result
+// does not depend on their timing.
+template <int TOKENS>
+struct SlotTable {
+  static constexpr int kSize = 2 * TOKENS;
+  long long slot[TOKENS];   // slots of the CTA's tokens; -1: nothing is written
+  int head[kSize];          // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
+  int dead[TOKENS];         // a later token writes the same slot
+};
+
+__device__ __forceinline__ uint32_t slot_hash(long long s) {
+  uint32_t h = (uint32_t)s ^ (uint32_t)(s >> 32) * 0x9E3779B1u;
+  h *= 0x85EBCA6Bu;
+  return h ^ (h >> 15);
+}
+
+template <typename T, bool MXF>
+__device__ __forceinline__ void encode_row(const Side& sd, long long token, long long slot, int head, int heads, int dim,
+                                           int group, int sub, uint32_t lanes) {
+  // `group` lanes (a power of two) hold a row of one head, eight values at a time
+  const T* x = reinterpret_cast<const T*>(sd.x) + token * sd.x_token + head * sd.x_head;
+  const int chunks = dim / 8;
+  const size_t row = (size_t)slot * heads + head;
+  if (MXF) {
+    for (int c0 = 0; c0 < chunks; c0 += group) {  // every lane of the group takes every step (shuffles)
+      const int c = c0 + sub;
+      Chunk<T> v;
+      const bool ok = c < chunks;
+      if (ok) v.load(x + c * 8);
+      else v.clear();
+      uint32_t amax = v.amax_bits();
+      amax = max(amax, __shfl_xor_sync(lanes, amax, 1));
+      amax = max(amax, __shfl_xor_sync(lanes, amax, 2));
+      const uint32_t byte = mx::scale_byte(amax);
+      float f[8];
+      v.values(f);
+      const float inv = mx::inverse_scale(byte);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
+      if (ok) {
+        reinterpret_cast<uint32_t*>(sd.codes + row * (dim / 2))[c] = byte == 255u ? 0u : mx::encode8(f);
+        if ((c & 3) == 0) sd.scales[row * (dim / 32) + c / 4] = (uint8_t)byte;
+      }
+    }
+  } else {
+    uint32_t amax = 0;
+    for (int c = sub; c < chunks; c += group) {
+      Chunk<T> v;
+      v.load(x + c * 8);
+      amax = max(amax, v.amax_bits());
+    }
+    for (int o = group >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(lanes, amax, o));
+    // the arithmetic of the per-token encode on the grid [-128, 127]; a row that holds a NaN or an
+    // infinity has no scale and reads back as NaN
+    const float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu)
+                                            : fmaxf(__fdiv_rn(__uint_as_float(amax), 127.5f), 1e-8f);
+    const Divisor d = make_divisor(scale);
+    for (int c = sub; c < chunks; c += group) {
+      Chunk<T> v;
+      v.load(x + c * 8);
+      float f[8];
+      v.values(f);
+      uint32_t w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x4[4] = {f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]};
+        float q[4];
+        code4_f32(x4, d, 0.0f, -128.0f, 127.0f, q);
+        w[h] = pack4_s8(q);
+      }
+      reinterpret_cast<uint2*>(sd.codes + row * dim)[c] = make_uint2(w[0], w[1]);
+    }
+    if (sub == 0) reinterpret_cast<float*>(sd.scales)[row] = scale;
+  }
+}
+
+template <typename T, bool MXF, int TOKENS>
+__global__ void __launch_bounds__(kThreads)
+kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, size_t tokens, long long n_slots,
+                int heads, int dim, int group, int32_t* status) {
+  __shared__ SlotTable<TOKENS> tab;
+  const size_t t0 = (size_t)blockIdx.x * TOKENS;
+  const int mine = (int)(tokens - t0 < (size_t)TOKENS ? tokens - t0 : (size_t)TOKENS);
+  for (int i = threadIdx.x; i < SlotTable<TOKENS>::kSize; i += kThreads) tab.head[i] = 0;
+  for (int i = threadIdx.x; i < mine; i += kThreads) {
+    long long s = index_at(slots, slot_bits, t0 + i);
+    if (s >= n_slots) {
+      s = -1;
+      if (status) atomicExch(status, (int)LQ_ERR_SHAPE);
+    }
+    tab.slot[i] = s < 0 ? -1 : s;
+    tab.dead[i] = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine; i += kThreads) {
+    const long long s = tab.slot[i];
+    if (s < 0) continue;
+    for (uint32_t h = slot_hash(s) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
+      const int old = atomicCAS(&tab.head[h], 0, i + 1);
+      if (old == 0) break;
+      if (tab.slot[old - 1] == s) {  // the entry stays with this slot: keep its latest token
+        const int was = atomicMax(&tab.head[h], i + 1);
+        tab.dead[was < i + 1 ? was - 1 : i] = 1;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kThreads) {
+    const long long s = index_at(slots, slot_bits, t);
+    if (s < 0) continue;
+    for (uint32_t h = slot_hash(s) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
+      const int e = tab.head[h];
+      if (e == 0) break;
+      if (tab.slot[e - 1] == s) {
+        tab.dead[e - 1] = 1;
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  // rows of this CTA: (token, head) of its share of the heads, keys then values
+  const int hs = (heads + gridDim.y - 1) / gridDim.y, h0 = blockIdx.y * hs, h1 = min(heads, h0 + hs);
+  if (h0 >= h1) return;
+  const int per = h1 - h0, lane = threadIdx.x & 31;
+  const int sub = lane & (group - 1);
+  const uint32_t lanes = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (lane & ~(group - 1));
+  const int rows = mine * per * 2;
+  for (int r = (int)threadIdx.x / group; r < rows; r += kThreads / group) {
+    const int side = r & 1, i = (r >> 1) / per, head = h0 + (r >> 1) % per;
+    if (tab.slot[i] < 0 || tab.dead[i]) continue;
+    encode_row<T, MXF>(side ? v : k, (long long)(t0 + i), tab.slot[i], head, heads, dim, group, sub, lanes);
+  }
+}
+
+// ---- read ----------------------------------------------------------------------------------------------
+
+template <typename T, bool MXF>
+__global__ void __launch_bounds__(kThreads)
+kv_read_kernel(const Side k, const Side v, long long n_pages, int page, int heads, int dim, const int* __restrict__ table,
+               long long table_stride, int max_blocks, const int* __restrict__ cu, const int* __restrict__ starts, int seqs,
+               size_t total, int clear_tail, int32_t* status) {
+  const size_t r = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  if (r >= total) return;
+  const int lane = threadIdx.x & 31;
+  // the sequence whose rows [cu[b], cu[b + 1]) hold r
+  int lo = 0, hi = seqs;  // first index in [0, seqs] with cu[index] > r
+  bool covered = (long long)r < (long long)__ldg(cu + seqs) && (long long)r >= (long long)__ldg(cu);
+  if (!covered && !clear_tail) return;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if ((long long)__ldg(cu + mid) > (long long)r) hi = mid;
+    else lo = mid + 1;
+  }
+  long long slot = -1;
+  if (covered && lo > 0) {
+    const int b = lo - 1;
+    const long long pos = (long long)r - __ldg(cu + b) + (starts ? __ldg(starts + b) : 0);
+    const long long blk = pos / page;
+    if (pos >= 0 && blk < max_blocks) {
+      const long long p = __ldg(table + b * table_stride + blk);
+      if (p >= 0 && p < n_pages) slot = p * page + pos % page;
+    }
+    if (slot < 0 && status && lane == 0) atomicExch(status, (int)LQ_ERR_SHAPE);
+  }
+  const int per_head = dim / 8;
+  for (int c = lane; c < heads * per_head * 2; c += 32) {
+    const int side = c / (heads * per_head), cc = c - side * heads * per_head;
+    const int head = cc / per_head, d0 = (cc - head * per_head) * 8;
+    const Side& sd = side ? v : k;
+    float f[8];
+    if (slot < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+    } else {
+      const size_t row = (size_t)slot * heads + head;
+      float s;
+      if (MXF) {
+        mx::decode8(__ldg(reinterpret_cast<const uint32_t*>(sd.codes + row * (dim / 2) + d0 / 2)), f);
+        s = mx::scale_value(__ldg(sd.scales + row * (dim / 32) + d0 / 32));
+      } else {
+        const int2 w = __ldg(reinterpret_cast<const int2*>(sd.codes + row * dim + d0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w.x >> (8 * i)), f[4 + i] = (float)(int8_t)(w.y >> (8 * i));
+        s = __ldg(reinterpret_cast<const float*>(sd.scales) + row);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], s);
+    }
+    mx::store8(reinterpret_cast<T*>(sd.out) + (long long)r * sd.out_token + head * sd.out_head + d0, f);
+  }
+}
+
+int check_format(const std::string& w, int format, size_t heads, size_t dim) {
+  if (format != LQ_KV_INT8 && format != LQ_KV_MXFP4) return fail(LQ_ERR_UNSUPPORTED, w + ": unknown cache format");
+  if (heads == 0 || heads > 4096) return fail(LQ_ERR_SHAPE, w + ": between 1 and 4096 heads");
+  const size_t step = format == LQ_KV_INT8 ? 16 : 32;
+  if (dim == 0 || dim % step != 0 || dim > (size_t)kMaxDim)
+    return fail(LQ_ERR_SHAPE, w + ": head_dim must be a multiple of " + std::to_string(step) + ", at most " + std::to_string(kMaxDim));
+  return LQ_OK;
+}
+
+template <typename T, bool MXF, int TOKENS>
+int write_tokens(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
+                 int dim, int group, int32_t* status, cudaStream_t st) {
+  const size_t tiles = (tokens + TOKENS - 1) / TOKENS;
+  if (tiles > 0x7fffffffu) return fail(LQ_ERR_SHAPE, "lq_kv_write: too many tokens for one launch");
+  unsigned split = 1;
+  while (tiles * split < 2 * (size_t)kNumSMs && split < (unsigned)heads) split *= 2;
+  kv_write_kernel<T, MXF, TOKENS><<<dim3((unsigned)tiles, split), kThreads, 0, st>>>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status);
+  return check_cuda(cudaGetLastError(), "lq_kv_write launch");
+}
+template <typename T, bool MXF>
+int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
+                   int dim, int32_t* status, cudaStream_t st) {
+  int group = 1;
+  while (group < 32 && group * 8 < dim) group *= 2;
+  if (tokens <= 4096) return write_tokens<T, MXF, 16>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
+  if (tokens <= 32768) return write_tokens<T, MXF, 128>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
+  return write_tokens<T, MXF, 1024>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
+}
+
+}  // namespace
+}  // namespace lq
+
+using namespace lq;
+
+extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t tokens, size_t heads, size_t dim, size_t k_token,
+                           size_t k_head, size_t v_token, size_t v_head, const void* slots, int slot_bits, size_t n_slots, int format,
+                           void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t* status, void* stream) {
+  if (tokens == 0) return LQ_OK;
+  if (!k || !v || !slots || !k_codes || !k_scales || !v_codes || !v_scales) return fail(LQ_ERR_DEVICE, "lq_kv_write: null pointer");
+  if (in_dtype != LQ_F32 && in_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_kv_write: k and v must be f32|bf16");
+  if (slot_bits != 32 && slot_bits != 64) return fail(LQ_ERR_DTYPE, "lq_kv_write: slots must be int32 or int64");
+  if (int rc = check_format("lq_kv_write", format, heads, dim)) return rc;
+  const size_t esz = in_dtype == LQ_F32 ? 4 : 2;
+  if (!aligned16(k) || !aligned16(v) || (k_token * esz) % 16 || (k_head * esz) % 16 || (v_token * esz) % 16 || (v_head * esz) % 16)
+    return fail(LQ_ERR_ALIGNMENT, "lq_kv_write: rows of k and v must be 16-byte aligned");
+  if (!aligned16(k_codes) || !aligned16(v_codes) || !aligned16(k_scales) || !aligned16(v_scales))
+    return fail(LQ_ERR_ALIGNMENT, "lq_kv_write: the cache must be 16-byte aligned");
+  Side ks = {k, (long long)k_token, (long long)k_head, (uint8_t*)k_codes, (uint8_t*)k_scales, nullptr, 0, 0};
+  Side vs = {v, (long long)v_token, (long long)v_head, (uint8_t*)v_codes, (uint8_t*)v_scales, nullptr, 0, 0};
+  cudaStream_t st = (cudaStream_t)stream;
+  const int h = (int)heads, d = (int)dim;
+  if (in_dtype == LQ_F32)
+    return format == LQ_KV_MXFP4 ? write_dispatch<float, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st)
+                                 : write_dispatch<float, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st);
+  return format == LQ_KV_MXFP4 ? write_dispatch<bf16, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st)
+                               : write_dispatch<bf16, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st);
+}
+
+extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int format,
+                          size_t n_pages, size_t page, size_t heads, size_t dim, const int32_t* table, size_t table_stride,
+                          size_t max_blocks, const int32_t* cu_seqlens, const int32_t* starts, size_t seqs, size_t total,
+                          void* out_k, void* out_v, int out_dtype, size_t k_token, size_t k_head, size_t v_token, size_t v_head,
+                          int clear_tail, int32_t* status, void* stream) {
+  if (total == 0) return LQ_OK;
+  if (!k_codes || !k_scales || !v_codes || !v_scales || !out_k || !out_v || !cu_seqlens || (!table && max_blocks > 0))
+    return fail(LQ_ERR_DEVICE, "lq_kv_read: null pointer");
+  if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_kv_read: out must be f32|bf16");
+  if (int rc = check_format("lq_kv_read", format, heads, dim)) return rc;
+  if (page == 0 || page >= ((size_t)1 << 31) || seqs >= ((size_t)1 << 31) || max_blocks >= ((size_t)1 << 31))
+    return fail(LQ_ERR_SHAPE, "lq_kv_read: page size, sequences and table width must fit 32 bits, the page not empty");
+  if (total >= ((size_t)1 << 31)) return fail(LQ_ERR_SHAPE, "lq_kv_read: at most 2^31 - 1 rows");
+  const size_t esz = out_dtype == LQ_F32 ? 4 : 2;
+  if (!aligned16(out_k) || !aligned16(out_v) || (k_token * esz) % 16 || (k_head * esz) % 16 || (v_token * esz) % 16 || (v_head * esz) % 16)
+    return fail(LQ_ERR_ALIGNMENT, "lq_kv_read: output rows must be 16-byte aligned");
+  if (!aligned16(k_codes) || !aligned16(v_codes) || !aligned16(k_scales) || !aligned16(v_scales))
+    return fail(LQ_ERR_ALIGNMENT, "lq_kv_read: the cache must be 16-byte aligned");
+  Side ks = {nullptr, 0, 0, (uint8_t*)k_codes, (uint8_t*)k_scales, out_k, (long long)k_token, (long long)k_head};
+  Side vs = {nullptr, 0, 0, (uint8_t*)v_codes, (uint8_t*)v_scales, out_v, (long long)v_token, (long long)v_head};
+  const unsigned grid = (unsigned)((total * 32 + kThreads - 1) / kThreads);
+  cudaStream_t st = (cudaStream_t)stream;
+#define LQ_KV_READ(T, F)                                                                                                        \
+  kv_read_kernel<T, F><<<grid, kThreads, 0, st>>>(ks, vs, (long long)n_pages, (int)page, (int)heads, (int)dim, table,            \
+                                                  (long long)table_stride, (int)max_blocks, cu_seqlens, starts, (int)seqs, total, \
+                                                  clear_tail, status)
+  if (out_dtype == LQ_F32) {
+    if (format == LQ_KV_MXFP4) LQ_KV_READ(float, true);
+    else LQ_KV_READ(float, false);
+  } else {
+    if (format == LQ_KV_MXFP4) LQ_KV_READ(bf16, true);
+    else LQ_KV_READ(bf16, false);
+  }
+#undef LQ_KV_READ
+  return check_cuda(cudaGetLastError(), "lq_kv_read launch");
+}

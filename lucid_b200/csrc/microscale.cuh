@@ -1,0 +1,140 @@
+// MXFP4 element and scale conversions shared by the microscaled kernels.
+//
+// A block of 32 values holds 4-bit floats (E2M1: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives) and one
+// power-of-two scale, kept as its biased exponent (E8M0, 255 = NaN).  The scale of a block is
+// 2^(floor(log2 amax) - 2), so the largest magnitude lands in [4, 8) of the element grid: 2 is the
+// exponent of the grid's largest value.  Scaling by a power of two is exact, so an element is rounded
+// once (ties to the even mantissa, clamped at 6).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace lq {
+namespace mx {
+
+constexpr int kBlock = 32;        // values per scale
+constexpr int kTileRows = 128;    // a scale tile: 128 rows x 8 blocks, 1024 bytes
+constexpr int kTileCols = 256;    // ... which cover 256 values of K
+constexpr int kTileBytes = 1024;
+
+// Byte of (row, block) inside its tile: two halves of four blocks, each 32 rows x 4 row groups x 4 blocks
+// (the order in which the tensor core's scale operand wants its lanes).
+__host__ __device__ __forceinline__ int tile_offset(int row, int block) {
+  return (block >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (block & 3);
+}
+
+// Scale byte of a block from the float32 bit pattern of its largest magnitude.  The exponent field is
+// floor(log2) + 127 for normal values; zero and subnormal blocks, and exponents below the format's
+// range, take byte 0 (2^-127); an infinity or NaN anywhere in the block takes byte 255.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  return e == 255u ? 255u : (e < 2u ? 0u : e - 2u);
+}
+// 1 / scale, exact (byte <= 252 whenever it came from finite float32 values)
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// The scale itself: byte 0 is the subnormal 2^-127, byte 255 NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : (byte == 255u ? 0x7fffffffu : byte << 23));
+}
+
+// Eight scaled values -> eight 4-bit codes, value i in bits [4i, 4i + 4).
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// Eight codes -> their values (exact in float16, and so in float32).
+__device__ __forceinline__ void decode8(uint32_t codes, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+
+// The element nearest to a scaled value (magnitude below 8), as a value.  The grid's spacing is 1/2 below
+// 2, 1 below 4 and 2 above; adding and subtracting 1.5 * 2^23 spacings rounds to a multiple of it, ties to
+// the even multiple, which is the even mantissa.  (encode8 followed by decode8 in one kernel came out as
+// zeros from this toolchain; through memory the pair is right.)
+__device__ __forceinline__ float round_element(float t) {
+  const float a = fabsf(t);
+  const float m = a < 2.0f ? 6291456.0f : (a < 4.0f ? 12582912.0f : 25165824.0f);
+  return copysignf(fminf(__fsub_rn(__fadd_rn(a, m), m), 6.0f), t);
+}
+
+// Eight consecutive values of a thread, kept as they were loaded.
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  }
+  __device__ __forceinline__ void clear() { a = b = make_uint4(0, 0, 0, 0); }
+  // float32 bit pattern of the largest magnitude (ordered like the magnitudes, NaN above infinity)
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(max(a.x & m, a.y & m), max(a.z & m, a.w & m)), max(max(b.x & m, b.y & m), max(b.z & m, b.w & m)));
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+  }
+};
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <>
+struct Chunk<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void clear() { a = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t t = max_u16x2(max_u16x2(a.x & m, a.y & m), max_u16x2(a.z & m, a.w & m));
+    return max(t << 16, t & 0xffff0000u);
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+};
+
+// Eight values -> memory (16-byte aligned), rounded once when T is narrower.
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7]));
+}
+
+}  // namespace mx
+}  // namespace lq

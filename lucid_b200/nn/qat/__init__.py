@@ -11,4 +11,5 @@ from .modules import (  # noqa: F401
     Embedding,
     Linear,
     LinearReLU,
+    MXLinear,
 )

@@ -11,6 +11,9 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from ..._lib import ShapeMismatch
+from ...quantization._mx import mx_fake_quantize
+
 
 def _inner_of(mod):
     """A fused float container (``nni.LinearReLU`` / ``nni.ConvReLU*d``) hands over its first
@@ -51,6 +54,32 @@ class Linear(torch.nn.Linear):
 
 class LinearReLU(Linear):
     _RELU = True
+
+
+class MXLinear(torch.nn.Linear):
+    """A float Linear trained against the microscaled 4-bit format: input and weight each go through
+    ``mx_fake_quantize`` (straight-through gradients), so its forward is that of
+    ``nn.quantized.MXLinear`` up to the order of the sums.  Nothing is observed."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, relu: bool = False, **kw) -> None:
+        super().__init__(in_features, out_features, bias, **kw)
+        if in_features <= 0 or in_features % 32 != 0:
+            raise ShapeMismatch(f"in_features must be a multiple of 32, got {in_features}")
+        self.relu = relu
+        self.activation_post_process = torch.nn.Identity()  # ``convert`` takes what carries one
+
+    def forward(self, x):
+        y = F.linear(mx_fake_quantize(x), mx_fake_quantize(self.weight), self.bias)
+        return F.relu(y) if self.relu else y
+
+    @classmethod
+    def from_float(cls, mod, relu: bool = False) -> "MXLinear":
+        qat = cls(mod.in_features, mod.out_features, bias=mod.bias is not None, relu=relu,
+                  device=mod.weight.device, dtype=mod.weight.dtype)
+        qat.weight = mod.weight
+        if mod.bias is not None:
+            qat.bias = mod.bias
+        return qat
 
 
 class _ConvMixin:

@@ -4,6 +4,8 @@ affine primitives and the calibration observers."""
 
 from ._functional import (dequantize, fake_quantize, quantize, quantize_dynamic_per_tensor,  # noqa: F401
                           quantize_per_token, quantize_to)
+from ._kv_cache import KVCache, kv_cache_alloc, kv_cache_read, kv_cache_write  # noqa: F401
+from ._mx import mx_dequantize, mx_fake_quantize, mx_linear, mx_matmul, mx_quantize  # noqa: F401
 from ._qparams import QParams, calculate_qparams  # noqa: F401
 from ._qscheme import (QDtype, QScheme, per_channel_affine, per_channel_symmetric,  # noqa: F401
                        per_tensor_affine, per_tensor_symmetric, qint4, qint8, qint32, quint8)

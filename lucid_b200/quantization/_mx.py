@@ -1,0 +1,194 @@
+"""Microscaled 4-bit floating point (MXFP4): quantization, its inverse, the fake quantization of
+training, and the product on the 4-bit tensor cores.
+
+Blocks of 32 values along the last axis share one power-of-two scale; an element is one of 0, 0.5, 1,
+1.5, 2, 3, 4, 6 or its negative (``include/lucid_b200.h`` states the rounding and the layouts).  Unlike the
+affine grids there is nothing to calibrate: a scale is the exponent of its block's largest magnitude, so
+weights and activations are encoded by the same call, activations on every forward.
+
+``mx_quantize`` returns ``(codes, scales)``: ``codes`` is uint8 ``(..., K / 2)``, two elements a byte, and
+``scales`` uint8 ``(ceil(rows / 128), ceil(K / 256), 1024)``, the scale bytes in the tiles the tensor cores
+read (``rows`` being the product of the leading axes)."""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _float_input(x, what: str) -> torch.Tensor:
+    _lib.require_cuda(x, what)
+    if x.dtype not in _FLOATS:
+        raise _lib.DtypeMismatch(f"{what} must be float32 or bfloat16, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 32 != 0:
+        raise _lib.ShapeMismatch(f"{what} needs a last axis that is a multiple of 32, got {tuple(x.shape)}")
+    return x.detach()
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as (rows, K) with unit column stride and 16-byte aligned rows, copied only if it has to be."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    step = 16 // x2.element_size()
+    if x2.stride(1) != 1 or x2.stride(0) % step or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _dense(x: torch.Tensor) -> torch.Tensor:
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def _scale_shape(rows: int, k: int) -> tuple:
+    return ((rows + 127) // 128, (k + 255) // 256, 1024)
+
+
+def _check_packed(codes, scales, what: str) -> tuple:
+    """``(codes, scales, rows, K)`` of a packed matrix, its two tensors checked against each other."""
+    for t, name in ((codes, "codes"), (scales, "scales")):
+        _lib.require_cuda(t, f"{what} {name}")
+        if t.dtype != torch.uint8:
+            raise _lib.DtypeMismatch(f"{what} {name} must be uint8, got {t.dtype}")
+    if scales.device != codes.device:
+        raise _lib.DeviceMismatch(f"{what}: codes on {codes.device}, scales on {scales.device}")
+    if codes.dim() == 0 or codes.shape[-1] == 0 or codes.shape[-1] % 16 != 0:
+        raise _lib.ShapeMismatch(f"{what} codes need a last axis that is a multiple of 16, got {tuple(codes.shape)}")
+    k = codes.shape[-1] * 2
+    rows = codes.numel() * 2 // k
+    if tuple(scales.shape) != _scale_shape(rows, k):
+        raise _lib.ShapeMismatch(f"{what} scales are {tuple(scales.shape)}, expected {_scale_shape(rows, k)}")
+    return _dense(codes), _dense(scales), rows, k
+
+
+def mx_quantize(x: torch.Tensor):
+    """``(codes, scales)`` of ``x`` (float32 or bfloat16, the last axis a multiple of 32).  A block with
+    a NaN or an infinity decodes to NaN."""
+    x = _float_input(x, "mx_quantize input")
+    x2 = _rows(x)
+    rows, k = x2.shape
+    codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_shape(rows, k), dtype=torch.uint8, device=x.device)
+    _lib.call("lq_mx_quantize", x.device, x2.data_ptr(), _lib.code_of(x2.dtype), rows, k, x2.stride(0), codes.data_ptr(),
+          scales.data_ptr())
+    return codes, scales
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values ``(codes, scales)`` stand for: exact in float32 and in bfloat16."""
+    if out_dtype not in _FLOATS:
+        raise _lib.DtypeMismatch(f"mx_dequantize writes float32 or bfloat16, got {out_dtype}")
+    c, s, rows, k = _check_packed(codes, scales, "mx_dequantize")
+    out = torch.empty((*codes.shape[:-1], k), dtype=out_dtype, device=codes.device)
+    _lib.call("lq_mx_dequantize", codes.device, c.data_ptr(), s.data_ptr(), rows, k, out.data_ptr(), _lib.code_of(out_dtype))
+    return out
+
+
+class _StraightThrough(torch.autograd.Function):
+    """The gradient of the fake quantization: linear in the gradient that comes in, so it is its own
+    derivative."""
+
+    @staticmethod
+    def forward(ctx, grad, mask):
+        ctx.save_for_backward(mask)
+        g = _dense(grad.detach())
+        out = torch.empty_like(g)
+        _lib.call("lq_mx_fake_quantize_grad", g.device, g.data_ptr(), _lib.code_of(g.dtype), mask.data_ptr(), g.numel(),
+              out.data_ptr())
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        (mask,) = ctx.saved_tensors
+        return _StraightThrough.apply(grad, mask), None
+
+
+def _fake_quantize(x: torch.Tensor, want_mask: bool):
+    xc = _dense(_float_input(x, "mx_fake_quantize input"))
+    out = torch.empty_like(xc)
+    mask = torch.empty(xc.numel() // 8, dtype=torch.uint8, device=xc.device) if want_mask else None
+    _lib.call("lq_mx_fake_quantize", xc.device, xc.data_ptr(), _lib.code_of(xc.dtype), xc.numel(), out.data_ptr(), _addr(mask))
+    return out, mask
+
+
+class _MXFakeQuantize(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        out, mask = _fake_quantize(x, True)
+        ctx.save_for_backward(mask)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        (mask,) = ctx.saved_tensors
+        return _StraightThrough.apply(grad, mask)
+
+
+def mx_fake_quantize(x: torch.Tensor) -> torch.Tensor:
+    """``mx_dequantize(*mx_quantize(x))`` in one pass, in ``x``'s dtype, with the straight-through
+    gradient: it passes where the element was rounded inside the grid and is zero where it was clamped
+    (and in blocks that decode to NaN)."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        return _MXFakeQuantize.apply(x)
+    return _fake_quantize(x, False)[0]
+
+
+def _bias_of(bias, n: int, device) -> torch.Tensor | None:
+    if bias is None:
+        return None
+    _lib.require_cuda(bias, "bias")
+    if bias.device != device:
+        raise _lib.DeviceMismatch(f"bias on {bias.device}, the product runs on {device}")
+    if tuple(bias.shape) != (n,):
+        raise _lib.ShapeMismatch(f"bias is {tuple(bias.shape)}, expected {(n,)}")
+    return bias.detach().to(torch.float32).contiguous()
+
+
+def mx_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
+              bias: torch.Tensor | None = None, relu: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``a @ w.T (+ bias)`` of two packed matrices, ``a`` ``(..., K)`` and ``w`` ``(N, K)``, with float32
+    accumulation; float32 or bfloat16 out."""
+    if out_dtype not in _FLOATS:
+        raise _lib.DtypeMismatch(f"mx_matmul writes float32 or bfloat16, got {out_dtype}")
+    ac, sa, m, k = _check_packed(a_codes, a_scales, "mx_matmul left operand")
+    wc, sw, n, kw = _check_packed(w_codes, w_scales, "mx_matmul weight")
+    if w_codes.dim() != 2:
+        raise _lib.ShapeMismatch(f"the weight's codes must be (N, K / 2), got {tuple(w_codes.shape)}")
+    if k != kw:
+        raise _lib.ShapeMismatch(f"the left operand has {k} features, the weight {kw}")
+    if w_codes.device != a_codes.device:
+        raise _lib.DeviceMismatch(f"left operand on {a_codes.device}, weight on {w_codes.device}")
+    b = _bias_of(bias, n, a_codes.device)
+    out = torch.empty((*a_codes.shape[:-1], n), dtype=out_dtype, device=a_codes.device)
+    _lib.call("lq_mx_matmul", a_codes.device, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
+          int(relu), out.data_ptr(), _lib.code_of(out_dtype), n, _lib.status_word(a_codes.device).data_ptr())
+    return out
+
+
+def mx_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None = None,
+              relu: bool = False) -> torch.Tensor:
+    """``mx_matmul(*mx_quantize(x), ...)`` in one call; the result has ``x``'s dtype."""
+    x = _float_input(x, "mx_linear input")
+    wc, sw, n, k = _check_packed(w_codes, w_scales, "mx_linear weight")
+    if w_codes.dim() != 2:
+        raise _lib.ShapeMismatch(f"the weight's codes must be (N, K / 2), got {tuple(w_codes.shape)}")
+    if x.shape[-1] != k:
+        raise _lib.ShapeMismatch(f"the input has {x.shape[-1]} features, the weight {k}")
+    if w_codes.device != x.device:
+        raise _lib.DeviceMismatch(f"input on {x.device}, weight on {w_codes.device}")
+    b = _bias_of(bias, n, x.device)
+    x2 = _rows(x)
+    m = x2.shape[0]
+    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    room = (m * (k // 2) + 1023) // 1024 * 1024 + (m + 127) // 128 * ((k + 255) // 256) * 1024
+    ws = torch.empty(room, dtype=torch.uint8, device=x.device)
+    code = _lib.code_of(x.dtype)
+    _lib.call("lq_mx_linear", x.device, x2.data_ptr(), code, m, x2.stride(0), wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
+          int(relu), out.data_ptr(), code, n, ws.data_ptr(), room, _lib.status_word(x.device).data_ptr())
+    return out

@@ -140,8 +140,13 @@ def _quant_mapping() -> dict:
     for cls in (nniqat.ConvBn1d, nniqat.ConvBn2d, nniqat.ConvBn3d,
                 nniqat.ConvBnReLU1d, nniqat.ConvBnReLU2d, nniqat.ConvBnReLU3d):
         m[cls] = lambda mod: mod.to_quantized()
+    m[nnqat.MXLinear] = lambda mod: nnq.MXLinear.from_float(mod, relu=mod.relu)
     from .. import backends
 
+    if backends.quantized.use_mx():  # the Linear family on microscaled 4-bit floats
+        m[torch.nn.Linear] = _mx_linear_builder(False)
+        if nni is not None:
+            m[nni.LinearReLU] = _mx_linear_builder(True)
     if backends.quantized.use_mlx():  # the Linear family on the group-wise weight-only kernel
         m[torch.nn.Linear] = _mlx_linear_builder(False)
         if nni is not None:
@@ -196,6 +201,43 @@ def _mlx_dynamic_builder():
         if gs is None or dtype.bits not in (4, 8):
             return nnq.dynamic.Linear.from_float(child, dtype)
         return nnq.QuantizedLinearMLX.from_float(child, bits=dtype.bits, group_size=gs, relu=False)
+
+    return build
+
+
+def _mx_linear_builder(relu: bool):
+    """``convert`` builder of the microscaled route: a layer whose width is no multiple of the block
+    size falls back to the calibrated layer."""
+    import lucid_b200.nn.quantized as nnq
+
+    fallback = nnq.LinearReLU.from_float if relu else nnq.Linear.from_float
+
+    def build(child):
+        inner = child[0] if relu else child
+        return fallback(child) if inner.in_features % 32 else nnq.MXLinear.from_float(inner, relu=relu)
+
+    return build
+
+
+def _mx_dynamic_builder():
+    """``quantize_dynamic`` builder of the microscaled route."""
+    import lucid_b200.nn.quantized as nnq
+
+    def build(child, dtype):
+        return nnq.dynamic.Linear.from_float(child, dtype) if child.in_features % 32 else nnq.MXLinear.from_float(child)
+
+    return build
+
+
+def _mx_qat_builder(relu: bool):
+    """``prepare_qat`` builder of the microscaled route."""
+    from ..nn import qat as nnqat
+
+    fallback = nnqat.LinearReLU.from_float if relu else nnqat.Linear.from_float
+
+    def build(child):
+        inner = child[0] if relu else child
+        return fallback(child) if inner.in_features % 32 else nnqat.MXLinear.from_float(inner, relu=relu)
 
     return build
 
@@ -299,6 +341,12 @@ def prepare_qat(model: torch.nn.Module, qconfig: QConfig | QConfigMapping | None
     if nni is not None:
         mapping.update({nni.LinearReLU: nnqat.LinearReLU.from_float, nni.ConvReLU1d: nnqat.ConvReLU1d.from_float,
                         nni.ConvReLU2d: nnqat.ConvReLU2d.from_float, nni.ConvReLU3d: nnqat.ConvReLU3d.from_float})
+    from .. import backends
+
+    if backends.quantized.use_mx():
+        mapping[torch.nn.Linear] = _mx_qat_builder(False)
+        if nni is not None:
+            mapping[nni.LinearReLU] = _mx_qat_builder(True)
     n_matched = 0
 
     from ..nn.intrinsic import qat as nniqat
@@ -344,7 +392,11 @@ def _dynamic_mapping() -> dict:
 
     from .. import backends
 
-    linear = _mlx_dynamic_builder() if backends.quantized.use_mlx() else nnq.dynamic.Linear.from_float
+    linear = nnq.dynamic.Linear.from_float
+    if backends.quantized.use_mlx():
+        linear = _mlx_dynamic_builder()
+    elif backends.quantized.use_mx():
+        linear = _mx_dynamic_builder()
     return {torch.nn.Linear: linear,
             torch.nn.LSTM: nnq.dynamic.LSTM.from_float,
             torch.nn.Embedding: lambda mod, dtype: nnq.Embedding.from_float(mod),

@@ -19,7 +19,7 @@ SOURCES = ["capi.cu", "stream_kernels.cu", "histogram.cu", "embedding.cu", "exch
            "gemm_s8.cu", "microscale.cu", "gemm_mx.cu", "kvcache.cu"]
 # the test-only library: the GEMM with its wait-expiry hook compiled in (-DLQ_TESTING)
 TEST_SOURCES = ["capi.cu", "gemm_s8.cu"]
-HEADERS = ["common.cuh", "microscale.cuh", os.path.join(ROOT, "include", "lucid_b200.h")]
+HEADERS = ["common.cuh", "microscale.cuh", "tcgen05.cuh", os.path.join(ROOT, "include", "lucid_b200.h")]
 LIB = os.path.join(HERE, "liblucid_b200.so")
 TEST_LIB = os.path.join(HERE, "liblucid_b200_testing.so")
 

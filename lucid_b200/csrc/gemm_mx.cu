@@ -1,42 +1,385 @@
-// Product of two MXFP4 matrices.
-//   out[m, n] = sum_k a[m, k] * w[n, k] (+ bias[n]) (ReLU), float32 accumulation.
+// Product of two MXFP4 matrices on the 4-bit tensor cores (sm_100a):
+//   out[m, n] = sum_k a[m, k] * w[n, k] (+ bias[n]) (ReLU), float32 accumulation in TMEM.
+//
+// tcgen05.mma kind::mxf4 multiplies the packed codes and applies both operands' block scales itself, so the
+// kernel moves bytes: codes by TMA (128 bytes = 256 values of K a row and stage, 128-byte swizzle), scale
+// tiles by TMA as they lie (1024 bytes = 128 rows x 256 values, which is why the encode writes them that
+// way), from shared memory into TMEM by tcgen05.cp.  The weight is the operand whose rows become TMEM
+// lanes (128 output features a CTA) and the activations the one whose rows become columns: a decode step
+// of a few tokens then pays for 16 columns instead of 128 rows, every lane owns one output feature and
+// its bias, and neighbouring lanes store neighbouring outputs.
+#include <string.h>
+
+#include <mutex>
+
 #include "microscale.cuh"
+#include "tcgen05.cuh"
 
 namespace lq {
 namespace {
 
+constexpr int kRows = 128;            // output features of a CTA
+constexpr int kStageK = 256;          // values of K per stage: one 128-byte swizzle row
+constexpr int kWBytes = kRows * 128;  // weight codes of a stage
+
+struct Args {
+  int M, N, num_kb;      // tokens, output features, stages of K
+  int tiles_t, tiles_f;
+  int split;             // CTAs (a cluster) that share the K axis of a tile
+  int early;             // the weight may be fetched before the preceding kernel has finished
+  const float* bias;
+  int relu;
+  void* out;
+  long long ldo;
+  int pairs_ok;          // two neighbouring bf16 outputs of a row share an aligned word
+  int quads_ok;          // four neighbouring outputs are one aligned store
+  int32_t* status;
+  long long budget;
+};
+
+// ---- PTX ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows x 16 bytes of shared memory -> four TMEM columns, the same in each of the four lane quadrants
+__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// 512 contiguous bytes as rows of 16 without swizzle: eight rows (128 bytes) a core matrix
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// Instruction descriptor: both operands E2M1 and K-major, scales UE8M0; `id` selects which two of the
+// four scale bytes of a column a multiply of 64 values uses (0 or 2).
+__device__ __forceinline__ constexpr uint32_t mx_idesc(int m, int n, int id) {
+  return ((uint32_t)id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
+         ((uint32_t)id << 29);
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// ---- epilogue ------------------------------------------------------------------------------------------
+__device__ __forceinline__ float finish(float v, float bias, bool has_bias, int relu) {
+  if (has_bias) v = __fadd_rn(v, bias);
+  return relu && v < 0.0f ? 0.0f : v;  // a NaN stays
+}
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// One output per thread, block by block: sum over a block of the element products (exact: at most
-// 32 * 36 in steps of 1/4), times the two scales.
-template <typename T>
-__global__ void __launch_bounds__(128)
-mx_matmul_kernel(const uint8_t* __restrict__ a, const uint8_t* __restrict__ sa, size_t M, const uint8_t* __restrict__ w,
-                 const uint8_t* __restrict__ sw, size_t N, size_t K, const float* __restrict__ bias, int relu,
-                 T* __restrict__ out, size_t ldo) {
-  const size_t n = (size_t)blockIdx.x * 128 + threadIdx.x;
-  if (n >= N) return;
-  const size_t col_tiles = (K + mx::kTileCols - 1) / mx::kTileCols;
-  for (size_t m = blockIdx.y; m < M; m += gridDim.y) {
-    float acc = 0.0f;
-    for (size_t b = 0; b < K / mx::kBlock; ++b) {
-      float dot = 0.0f;
-      for (int q = 0; q < 4; ++q) {
-        float va[8], vw[8];
-        mx::decode8(__ldg(reinterpret_cast<const uint32_t*>(a + m * (K / 2) + b * 16) + q), va);
-        mx::decode8(__ldg(reinterpret_cast<const uint32_t*>(w + n * (K / 2) + b * 16) + q), vw);
+// Sixteen tokens [t, t + 16) of this lane's feature.  A warp writes 32 neighbouring features of a token per
+// store.  In bf16 two lanes trade halves, so that each writes one word of two features (of the first or
+// second token of a pair): half as many store instructions.
+__device__ __forceinline__ void store_block(const Args& g, float (&y)[16], int t, int f, int lane, float*) {
+  float* out = reinterpret_cast<float*>(g.out) + (long long)t * g.ldo + f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf(va[i], vw[i], dot);
-      }
-      const float fa = mx::scale_value(sa[(m / 128 * col_tiles + b / 8) * mx::kTileBytes + mx::tile_offset((int)(m % 128), (int)(b % 8))]);
-      const float fw = mx::scale_value(sw[(n / 128 * col_tiles + b / 8) * mx::kTileBytes + mx::tile_offset((int)(n % 128), (int)(b % 8))]);
-      acc = fmaf(dot * fa, fw, acc);
+  for (int j = 0; j < 16; ++j)
+    if (f < g.N && t + j < g.M) out[j * g.ldo] = y[j];
+}
+__device__ __forceinline__ void store_block(const Args& g, float (&y)[16], int t, int f, int lane, __nv_bfloat16*) {
+  if (g.pairs_ok) {
+    const int odd = lane & 1;
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(g.out) + (long long)(t + odd) * g.ldo + (f - odd);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float theirs = __shfl_xor_sync(0xffffffffu, odd ? y[j] : y[j + 1], 1);
+      const uint32_t w = odd ? mx::bf16x2_bits(theirs, y[j + 1]) : mx::bf16x2_bits(y[j], theirs);
+      if (f < g.N && t + j + odd < g.M) *reinterpret_cast<uint32_t*>(out + j * g.ldo) = w;
     }
-    if (bias) acc += __ldg(bias + n);
-    if (relu) acc = acc < 0.0f ? 0.0f : acc;
-    store1(out + m * ldo + n, acc);
+  } else {
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(g.out) + (long long)t * g.ldo + f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (f < g.N && t + j < g.M) out[j * g.ldo] = __float2bfloat16_rn(y[j]);
   }
+}
+
+// ---- one tile per CTA, K shared by a cluster --------------------------------------------------------------
+//
+// TN tokens x 128 features a CTA.  For few tokens the weight's stream from HBM is the bound: `split` CTAs of
+// a cluster each take a contiguous run of K, so that a narrow layer still occupies the GPU, and two CTAs
+// fit an SM, so that the copies of one run during the epilogue of the other.  The partial sums meet in
+// shared memory: every CTA reads the others' through the cluster and adds them in rank order (the same
+// result whatever the timing), each for its share of the outputs.
+constexpr int kThreads = 192;  // producer, multiply, four epilogue warps
+
+template <int TN>
+struct Cfg {
+  static constexpr int kXBytes = TN * 128;
+  static constexpr int kStageBytes = kWBytes + kXBytes + 2 * mx::kTileBytes;
+  static constexpr int kStages = TN <= 64 ? 4 : 3;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 128;
+  // TMEM: the accumulator, then two buffers of 8 + 8 scale columns (a power of two is allocated)
+  static constexpr int kTmemCols = TN + 32 <= 64 ? 64 : (TN + 32 <= 128 ? 128 : 256);
+  static_assert(2 * kSmemBytes <= 226 * 1024, "two CTAs share an SM");
+  static_assert(TN * kRows * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
+};
+
+template <int TN, typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+               const __grid_constant__ CUtensorMap tm_sw, const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ Args g) {
+  using C = Cfg<TN>;
+  extern __shared__ uint8_t smem_raw[];
+  // the same offset in every CTA of a cluster (the partial sums are read across it)
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* tail = smem + C::kStages * C::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail);  // full[S], empty[S], done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 96);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 100);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * C::kStages, bar_done = bar_empty + 8 * C::kStages;
+
+  const int tile = (int)blockIdx.x / g.split, rank = (int)blockIdx.x % g.split;
+  const int t0 = tile % g.tiles_t * TN, f0 = tile / g.tiles_t * kRows;
+  const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
+  const int n = kb1 - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2 * C::kStages + 1; ++s) mbar_init(bar_full + 8 * s, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_x) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_w = [&](int i) {
+        const int s = i % C::kStages, kb = kb0 + i;
+        const uint32_t dst = smem_u32(smem + s * C::kStageBytes), bar = bar_full + 8 * s;
+        mbar_expect_tx(bar, C::kStageBytes);
+        tma_load_2d(dst, &tm_w, kb * 128, f0, bar);
+        tma_load_3d(dst + kWBytes + C::kXBytes, &tm_sw, 0, kb, f0 / 128, bar);
+      };
+      // The weight does not depend on the kernel before this one (which encodes the activations): its first
+      // stages are on their way while that one still runs.
+      const int pre = g.early ? min(n, C::kStages) : 0;
+      for (int i = 0; i < pre; ++i) load_w(i);
+      pdl_wait();
+      pdl_launch_dependents();
+      for (int i = 0; i < n; ++i) {
+        const int s = i % C::kStages;
+        if (i >= C::kStages && !mbar_wait(bar_empty + 8 * s, (i / C::kStages - 1) & 1, abort_flag, g.budget)) break;
+        if (i >= pre) load_w(i);
+        const uint32_t dst = smem_u32(smem + s * C::kStageBytes), bar = bar_full + 8 * s;
+        tma_load_2d(dst + kWBytes, &tm_x, (kb0 + i) * 128, t0, bar);
+        tma_load_3d(dst + kWBytes + C::kXBytes + mx::kTileBytes, &tm_sx, 0, kb0 + i, t0 / 128, bar);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
+        const int s = i % C::kStages;
+        if (!mbar_wait(bar_full + 8 * s, (i / C::kStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+        // the scale columns of this buffer were last used two stages ago
+        if (i >= 2 && !mbar_wait(bar_empty + 8 * ((i - 2) % C::kStages), ((i - 2) / C::kStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t src = smem_u32(smem + s * C::kStageBytes);
+        const uint32_t ssrc = src + kWBytes + C::kXBytes;
+        const uint32_t sfw = tmem + TN + (i & 1) * 16, sfx = sfw + 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tc_cp_scales(sfw + 4 * h, scale_desc(ssrc + h * 512));
+          tc_cp_scales(sfx + 4 * h, scale_desc(ssrc + mx::kTileBytes + h * 512));
+        }
+        const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc_mma_mxf4(tmem, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(kRows, TN, 2 * (k & 1)), sfw + 4 * (k >> 1), sfx + 4 * (k >> 1),
+                      i | k ? 1u : 0u);
+        tc_commit(bar_empty + 8 * s);
+      }
+      if (ok) tc_commit(bar_done);
+    }
+    __syncwarp();
+  }
+  const bool epilogue = warp >= 2;
+  const int quad = warp & 3;
+  bool ok = true;
+  if (epilogue) {
+    pdl_wait();
+    ok = mbar_wait_warp<100>(bar_done, 0, abort_flag, g.budget);
+    tc_fence_after();
+  }
+  const int valid = min(TN, g.M - t0);
+  const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
+  if (g.split == 1) {
+    if (epilogue && ok) {
+      const int f = f0 + quad * 32 + lane;
+      const float b = g.bias && f < g.N ? __ldg(g.bias + f) : 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < valid; c += 16) {
+        uint32_t r[16];
+        tc_ld16_sync(taddr + c, r);
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[j] = finish(__uint_as_float(r[j]), b, g.bias != nullptr, g.relu);
+        store_block(g, y, t0 + c, f, lane, (T*)nullptr);
+      }
+    }
+  } else {
+    float* part = reinterpret_cast<float*>(smem);  // [token][feature]
+    if (epilogue && ok) {
+#pragma unroll 1
+      for (int c = 0; c < valid; c += 16) {
+        uint32_t r[16];
+        tc_ld16_sync(taddr + c, r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * kRows + quad * 32 + lane] = __uint_as_float(r[j]);
+      }
+    }
+    if (!epilogue) pdl_wait();
+    cluster_sync_all();
+    const int total = valid * kRows;
+    const int lo = (int)((long long)total * rank / g.split), hi = (int)((long long)total * (rank + 1) / g.split);
+    const uint32_t base = smem_u32(part);
+    for (int i = lo + (int)threadIdx.x; i < hi; i += kThreads) {
+      float v = 0.0f;
+      for (int r = 0; r < g.split; ++r) v = __fadd_rn(v, ld_cluster_f32(map_to_cta(base + 4 * i, r)));
+      const int f = f0 + i % kRows, t = t0 + i / kRows;
+      if (f < g.N && *abort_flag == 0)
+        store1(reinterpret_cast<T*>(g.out) + (long long)t * g.ldo + f, finish(v, g.bias ? __ldg(g.bias + f) : 0.0f, g.bias != nullptr, g.relu));
+    }
+    cluster_sync_all();  // nobody's partial sums go away while they are read
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    for (int i = 0; i < 50; ++i) __nanosleep(20000);  // copies and multiplies in flight land first
+    if (threadIdx.x == 0 && g.status) atomicExch(g.status, (int)LQ_ERR_TIMEOUT);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn get_encode() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      fn = (EncodeFn)p;
+  });
+  return fn;
+}
+// codes: (rows, K / 2) bytes, boxes of 128 bytes x box_rows, rows and bytes past the end read as zeros
+int code_map(CUtensorMap* tm, const void* base, size_t rows, size_t K, int box_rows) {
+  const cuuint64_t dims[2] = {K / 2, rows}, strides[1] = {K / 2};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+  const CUresult r = get_encode()(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_CUDA, "lq_mx_matmul: tensor map of the codes failed: " + std::to_string((int)r));
+}
+// scale tiles: (row tiles, column tiles, 256 words), boxes of one column tile x box_tiles row tiles
+int scale_map(CUtensorMap* tm, const void* base, size_t rows, size_t K, int box_tiles) {
+  const cuuint64_t ct = (K + kStageK - 1) / kStageK, rt = (rows + mx::kTileRows - 1) / mx::kTileRows;
+  const cuuint64_t dims[3] = {256, ct, rt}, strides[2] = {mx::kTileBytes, ct * mx::kTileBytes};
+  const cuuint32_t box[3] = {256, 1, (cuuint32_t)box_tiles}, ones[3] = {1, 1, 1};
+  const CUresult r = get_encode()(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, ones,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? LQ_OK : fail(LQ_ERR_CUDA, "lq_mx_matmul: tensor map of the scales failed: " + std::to_string((int)r));
+}
+
+struct Operands {
+  const uint8_t *x, *sx, *w, *sw;
+  size_t M, N, K;
+};
+
+template <int TN, typename T>
+int launch_tile(const Operands& o, Args g, cudaStream_t st) {
+  static PerDeviceOnce once;
+  using C = Cfg<TN>;
+  auto kernel = mx_tile_kernel<TN, T>;
+  const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); });
+  if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(max dynamic smem)");
+  g.tiles_t = (g.M + TN - 1) / TN, g.tiles_f = (g.N + kRows - 1) / kRows;
+  const long long tiles = (long long)g.tiles_t * g.tiles_f;
+  const long long room = 2ll * sm_count();
+  g.split = 1;
+  while (g.split < 8 && g.split < g.num_kb && tiles * (g.split + 1) <= room) ++g.split;
+  if (tiles * g.split > 0x7fffffffll) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: too many tiles for one launch");
+  CUtensorMap tw, tx, tsw, tsx;
+  if (int rc = code_map(&tw, o.w, o.N, o.K, kRows)) return rc;
+  if (int rc = code_map(&tx, o.x, o.M, o.K, TN)) return rc;
+  if (int rc = scale_map(&tsw, o.sw, o.N, o.K, 1)) return rc;
+  if (int rc = scale_map(&tsx, o.sx, o.M, o.K, 1)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * g.split)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = C::kSmemBytes, cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)g.split, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tw, tx, tsw, tsx, g), "lq_mx_matmul launch");
+}
+
+template <typename T>
+int launch(const Operands& o, const Args& g, cudaStream_t st) {
+  // the narrowest tile that holds all tokens: the rest of a wider one would be multiplied for nothing
+  if (o.M <= 16) return launch_tile<16, T>(o, g, st);
+  if (o.M <= 32) return launch_tile<32, T>(o, g, st);
+  if (o.M <= 64) return launch_tile<64, T>(o, g, st);
+  return launch_tile<128, T>(o, g, st);
+}
+
+int matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes, const uint8_t* w_scales, size_t N, size_t K,
+           const float* bias, int relu, void* out, int out_dtype, size_t ldo, int32_t* status, int early, cudaStream_t st) {
+  if (!a_codes || !a_scales || !w_codes || !w_scales || !out) return fail(LQ_ERR_DEVICE, "lq_mx_matmul: null pointer");
+  if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_mx_matmul: out must be f32|bf16");
+  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: K must be a multiple of 32");
+  if (M >= ((size_t)1 << 30) || N >= ((size_t)1 << 30) || K >= ((size_t)1 << 30)) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: extents must be below 2^30");
+  if (ldo < N) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: output row stride shorter than a row");
+  if (!aligned16(a_codes) || !aligned16(a_scales) || !aligned16(w_codes) || !aligned16(w_scales))
+    return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: codes and scales must be 16-byte aligned");
+  const size_t esz = out_dtype == LQ_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(out) % esz != 0) return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: out must be aligned to its type");
+  if (!get_encode()) return fail(LQ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  Args g;
+  memset(&g, 0, sizeof(g));
+  g.M = (int)M, g.N = (int)N, g.num_kb = (int)((K + kStageK - 1) / kStageK);
+  g.early = early, g.bias = bias, g.relu = relu, g.out = out, g.ldo = (long long)ldo, g.status = status, g.budget = kWaitBudgetCycles;
+  g.pairs_ok = out_dtype == LQ_BF16 && reinterpret_cast<uintptr_t>(out) % 4 == 0 && ldo % 2 == 0 && N % 2 == 0;
+  const Operands o = {a_codes, a_scales, w_codes, w_scales, M, N, K};
+  return out_dtype == LQ_F32 ? launch<float>(o, g, st) : launch<__nv_bfloat16>(o, g, st);
 }
 
 }  // namespace
@@ -52,21 +395,7 @@ extern "C" int lq_mx_matmul(const uint8_t* a_codes, const uint8_t* a_scales, siz
                             const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
                             int out_dtype, size_t ldo, int32_t* status, void* stream) {
   if (M == 0 || N == 0) return LQ_OK;
-  if (!a_codes || !a_scales || !w_codes || !w_scales || !out) return fail(LQ_ERR_DEVICE, "lq_mx_matmul: null pointer");
-  if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_mx_matmul: out must be f32|bf16");
-  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: K must be a multiple of 32");
-  if (M >= ((size_t)1 << 30) || N >= ((size_t)1 << 30) || K >= ((size_t)1 << 30)) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: extents must be below 2^30");
-  if (ldo < N) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: output row stride shorter than a row");
-  if (!aligned16(a_codes) || !aligned16(a_scales) || !aligned16(w_codes) || !aligned16(w_scales))
-    return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: codes and scales must be 16-byte aligned");
-  (void)status;
-  const dim3 grid((unsigned)((N + 127) / 128), (unsigned)(M < 4096 ? M : 4096));
-  cudaStream_t st = (cudaStream_t)stream;
-  if (out_dtype == LQ_F32)
-    mx_matmul_kernel<float><<<grid, 128, 0, st>>>(a_codes, a_scales, M, w_codes, w_scales, N, K, bias, relu, (float*)out, ldo);
-  else
-    mx_matmul_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a_codes, a_scales, M, w_codes, w_scales, N, K, bias, relu, (__nv_bfloat16*)out, ldo);
-  return check_cuda(cudaGetLastError(), "lq_mx_matmul launch");
+  return matmul(a_codes, a_scales, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status, 0, (cudaStream_t)stream);
 }
 
 extern "C" int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
@@ -74,9 +403,9 @@ extern "C" int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, c
                             uint8_t* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   if (M == 0 || N == 0) return LQ_OK;
   if (!workspace) return fail(LQ_ERR_DEVICE, "lq_mx_linear: null workspace");
-  if (K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_linear: K must be a multiple of 32");
+  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_linear: K must be a multiple of 32");
   if (workspace_bytes < lq_mx_linear_workspace_bytes(M, K)) return fail(LQ_ERR_WORKSPACE, "lq_mx_linear: workspace too small");
   uint8_t* a_scales = workspace + (M * (K / 2) + 1023) / 1024 * 1024;
   if (int rc = lq_mx_quantize(x, in_dtype, M, K, ldx, workspace, a_scales, stream)) return rc;
-  return lq_mx_matmul(workspace, a_scales, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status, stream);
+  return matmul(workspace, a_scales, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status, 1, (cudaStream_t)stream);
 }

@@ -42,6 +42,8 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 mx_quantize_kernel(const T* __restrict__ x, size_t rows, size_t K, size_t ldx, uint32_t col_tiles, size_t units,
                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  pdl_wait();
+  pdl_launch_dependents();
   const size_t unit = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   if (unit >= units) return;
   const int lane = threadIdx.x & 31;
@@ -158,9 +160,8 @@ extern "C" int lq_mx_quantize(const void* x, int in_dtype, size_t rows, size_t K
   const size_t grid = (units * 32 + kThreads - 1) / kThreads;
   if (int rc = check_grid("lq_mx_quantize", grid)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (in_dtype == LQ_F32) mx_quantize_kernel<float><<<(unsigned)grid, kThreads, 0, st>>>((const float*)x, rows, K, ldx, ct, units, codes, scales);
-  else mx_quantize_kernel<bf16><<<(unsigned)grid, kThreads, 0, st>>>((const bf16*)x, rows, K, ldx, ct, units, codes, scales);
-  return check_cuda(cudaGetLastError(), "lq_mx_quantize launch");
+  if (in_dtype == LQ_F32) return check_cuda(launch_pdl(mx_quantize_kernel<float>, dim3((unsigned)grid), dim3(kThreads), 0, st, (const float*)x, rows, K, ldx, ct, units, codes, scales), "lq_mx_quantize launch");
+  return check_cuda(launch_pdl(mx_quantize_kernel<bf16>, dim3((unsigned)grid), dim3(kThreads), 0, st, (const bf16*)x, rows, K, ldx, ct, units, codes, scales), "lq_mx_quantize launch");
 }
 
 extern "C" int lq_mx_dequantize(const uint8_t* codes, const uint8_t* scales, size_t rows, size_t K, void* out,

@@ -45,6 +45,38 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm,
       "l"(tm), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(tm), "r"(x), "r"(y), "r"(z), "r"(cluster_bar)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_mxf4_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                 uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// in both CTAs of the pair, each from its own shared memory
+__device__ __forceinline__ void tc_cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+__device__ __forceinline__ void tc_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld_dep8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
   asm volatile(
@@ -82,21 +114,23 @@ __device__ __forceinline__ float finish(float v, float bias, bool has_bias, int 
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Sixteen tokens [t, t + 16) of this lane's feature.  A warp writes 32 neighbouring features of a token per
+// COUNT tokens [t, t + COUNT) of this lane's feature.  A warp writes 32 neighbouring features of a token per
 // store.  In bf16 two lanes trade halves, so that each writes one word of two features (of the first or
 // second token of a pair): half as many store instructions.
-__device__ __forceinline__ void store_block(const Args& g, float (&y)[16], int t, int f, int lane, float*) {
+template <int COUNT>
+__device__ __forceinline__ void store_block(const Args& g, const float (&y)[COUNT], int t, int f, int lane, float*) {
   float* out = reinterpret_cast<float*>(g.out) + (long long)t * g.ldo + f;
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < COUNT; ++j)
     if (f < g.N && t + j < g.M) out[j * g.ldo] = y[j];
 }
-__device__ __forceinline__ void store_block(const Args& g, float (&y)[16], int t, int f, int lane, __nv_bfloat16*) {
+template <int COUNT>
+__device__ __forceinline__ void store_block(const Args& g, const float (&y)[COUNT], int t, int f, int lane, __nv_bfloat16*) {
   if (g.pairs_ok) {
     const int odd = lane & 1;
     __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(g.out) + (long long)(t + odd) * g.ldo + (f - odd);
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) {
+    for (int j = 0; j < COUNT; j += 2) {
       const float theirs = __shfl_xor_sync(0xffffffffu, odd ? y[j] : y[j + 1], 1);
       const uint32_t w = odd ? mx::bf16x2_bits(theirs, y[j + 1]) : mx::bf16x2_bits(y[j], theirs);
       if (f < g.N && t + j + odd < g.M) *reinterpret_cast<uint32_t*>(out + j * g.ldo) = w;
@@ -104,7 +138,7 @@ __device__ __forceinline__ void store_block(const Args& g, float (&y)[16], int t
   } else {
     __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(g.out) + (long long)t * g.ldo + f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int j = 0; j < COUNT; ++j)
       if (f < g.N && t + j < g.M) out[j * g.ldo] = __float2bfloat16_rn(y[j]);
   }
 }
@@ -241,7 +275,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         float y[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) y[j] = finish(__uint_as_float(r[j]), b, g.bias != nullptr, g.relu);
-        store_block(g, y, t0 + c, f, lane, (T*)nullptr);
+        store_block<16>(g, y, t0 + c, f, lane, (T*)nullptr);
       }
     }
   } else {
@@ -279,6 +313,176 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+// ---- CTA pairs, persistent ---------------------------------------------------------------------------------
+//
+// 256 features x 256 tokens per pair of CTAs (cta_group::2): each CTA stages its 128 weight rows and half of
+// the tokens, so a stage of 256 values of K moves 32 KB of codes into each SM for 512 cycles of multiplies --
+// half of what a lone 128 x 128 tile needs, whose operand traffic from L2 is its bound.  TMEM holds two
+// accumulators of 256 columns and two buffers of 24 scale columns only because the accumulators overlap:
+// columns 0..255 and 208..463, scales from 464.  The epilogue empties the 48 shared columns first and
+// says so on a barrier of their own; the next tile's multiplies then run while it works on the rest.
+constexpr int kPairTokens = 256;
+constexpr int kPairStages = 6;
+constexpr int kPairXBytes = kPairTokens / 2 * 128;
+constexpr int kPairStageBytes = kWBytes + kPairXBytes + 3 * mx::kTileBytes;
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 1024 + 256;
+constexpr int kPairEpilogueWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kPairEpilogueWarps;
+constexpr int kAccStep = 208, kAccShared = kPairTokens - kAccStep;  // columns between the accumulators, and shared
+constexpr int kScaleCols = 464;
+static_assert(kScaleCols >= kAccStep + kPairTokens && kScaleCols + 48 <= 512, "TMEM columns");
+static_assert(kPairSmemBytes <= 227 * 1024, "shared memory");
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+               const __grid_constant__ CUtensorMap tm_sw, const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ Args g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* tail = smem + kPairStages * kPairStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tail);  // full[S], empty[S], tfull[2], tempty[2], shared columns
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 192);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 196);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * kPairStages;
+  const uint32_t bar_tfull = bar_empty + 8 * kPairStages, bar_tempty = bar_tfull + 16, bar_shared = bar_tempty + 16;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int worker = (int)(blockIdx.x >> 1), workers = (int)(gridDim.x >> 1);
+  const int total = g.tiles_t * g.tiles_f;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2 * kPairStages + 2; ++s) mbar_init(bar_full + 8 * s, 1);
+    for (int s = 0; s < 3; ++s) mbar_init(bar_tempty + 8 * s, 2 * kPairEpilogueWarps);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_x) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < total; tile += workers) {
+        const int t0 = tile % g.tiles_t * kPairTokens, f0 = tile / g.tiles_t * 2 * kRows + (int)rank * kRows;
+        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
+          const int s = it % kPairStages;
+          if (it >= kPairStages && !mbar_wait(bar_empty + 8 * s, (it / kPairStages - 1) & 1, abort_flag, g.budget)) { ok = false; break; }
+          const uint32_t dst = smem_u32(smem + s * kPairStageBytes);
+          const uint32_t full = map_to_cta(bar_full + 8 * s, 0);  // both CTAs' bytes count on the leader's barrier
+          if (leader) mbar_expect_tx(bar_full + 8 * s, 2 * kPairStageBytes);
+          tma_load_2d_pair(dst, &tm_w, kb * 128, f0, full);
+          tma_load_2d_pair(dst + kWBytes, &tm_x, kb * 128, t0 + (int)rank * (kPairTokens / 2), full);
+          tma_load_3d_pair(dst + kWBytes + kPairXBytes, &tm_sw, 0, kb, f0 / 128, full);
+          tma_load_3d_pair(dst + kWBytes + kPairXBytes + mx::kTileBytes, &tm_sx, 0, kb, t0 / 128, full);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      int it = 0, q = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < total; tile += workers, ++q) {
+        const int acc = q & 1;
+        // this accumulator is empty, and so are the columns it shares with the one before
+        if (q >= 2 && !mbar_wait(bar_tempty + 8 * acc, ((q >> 1) - 1) & 1, abort_flag, g.budget)) break;
+        if (q >= 1 && !mbar_wait(bar_shared, (q - 1) & 1, abort_flag, g.budget)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * kAccStep;
+        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(bar_full + 8 * s, (it / kPairStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+          // the scale columns of this buffer were last used two stages ago
+          if (it >= 2 && !mbar_wait(bar_empty + 8 * ((it - 2) % kPairStages), ((it - 2) / kPairStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t src = smem_u32(smem + s * kPairStageBytes);
+          const uint32_t ssrc = src + kWBytes + kPairXBytes;
+          const uint32_t sfw = tmem + kScaleCols + (it & 1) * 24, sfx = sfw + 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tc_cp_scales_pair(sfw + 4 * h, scale_desc(ssrc + h * 512));
+            tc_cp_scales_pair(sfx + 8 * h, scale_desc(ssrc + mx::kTileBytes + h * 512));
+            tc_cp_scales_pair(sfx + 8 * h + 4, scale_desc(ssrc + 2 * mx::kTileBytes + h * 512));
+          }
+          const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_mxf4_pair(d, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(2 * kRows, kPairTokens, 2 * (k & 1)), sfw + 4 * (k >> 1),
+                             sfx + 8 * (k >> 1), kb | k ? 1u : 0u);
+          tc_commit_pair(bar_empty + 8 * s);
+        }
+        if (ok) tc_commit_pair(bar_tfull + 8 * acc);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tempty = map_to_cta(bar_tempty, 0), shared_cols = map_to_cta(bar_shared, 0);
+    int q = 0;
+    for (int tile = worker; tile < total; tile += workers, ++q) {
+      const int t0 = tile % g.tiles_t * kPairTokens;
+      const int f = tile / g.tiles_t * 2 * kRows + (int)rank * kRows + quad * 32 + lane;
+      const int acc = q & 1;
+      const float b = g.bias && f < g.N ? __ldg(g.bias + f) : 0.0f;
+      if (!mbar_wait_warp<100>(bar_tfull + 8 * acc, (q >> 1) & 1, abort_flag, g.budget)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + acc * kAccStep;
+      // [c0, c0 + 8 * blocks) of the tile's tokens, one block of eight read ahead
+      auto drain = [&](int c0, int blocks) {
+        uint32_t r[2][8];
+        tc_ld8(taddr + c0, r[0]);
+#pragma unroll 1
+        for (int i = 0; i < blocks; i += 2) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (i + u >= blocks) break;
+            tc_wait_ld_dep8(r[u]);
+            if (i + u + 1 < blocks) tc_ld8(taddr + c0 + 8 * (i + u + 1), r[u ^ 1]);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = finish(__uint_as_float(r[u][j]), b, g.bias != nullptr, g.relu);
+            if (t0 + c0 + 8 * (i + u) < g.M) store_block<8>(g, y, t0 + c0 + 8 * (i + u), f, lane, (T*)nullptr);
+          }
+        }
+      };
+      // columns 208..255 of TMEM: the last tokens of the first accumulator, the first of the second
+      drain((acc ? 0 : kAccStep) + half * (kAccShared / 2), kAccShared / 16);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(shared_cols);
+      drain((acc ? kAccShared : 0) + half * (kAccStep / 2), kAccStep / 16);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty + 8 * acc);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    for (int i = 0; i < 50; ++i) __nanosleep(20000);  // copies and multiplies in flight land first
+    if (threadIdx.x == 0 && g.status) atomicExch(g.status, (int)LQ_ERR_TIMEOUT);
+  }
+  cluster_sync_all();  // the peer may still signal this CTA's barriers or read its stages
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
@@ -353,7 +557,44 @@ int launch_tile(const Operands& o, Args g, cudaStream_t st) {
 }
 
 template <typename T>
+int launch_pair(const Operands& o, Args g, cudaStream_t st) {
+  static PerDeviceOnce once;
+  static int max_clusters[kMaxDevices] = {};
+  auto kernel = mx_pair_kernel<T>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sm_count()), cfg.blockDim = dim3(kPairThreads), cfg.dynamicSmemBytes = kPairSmemBytes, cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  const int dev = current_device();
+  const cudaError_t e = once.run([&]() -> cudaError_t {
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
+    int mc = 0;
+    if (err == cudaSuccess) err = cudaOccupancyMaxActiveClusters(&mc, kernel, &cfg);
+    max_clusters[dev] = mc > 0 ? mc : 1;
+    return err;
+  });
+  if (e != cudaSuccess) return check_cuda(e, "mx_pair_kernel setup");
+  g.split = 1;
+  g.tiles_t = (g.M + kPairTokens - 1) / kPairTokens, g.tiles_f = (g.N + 2 * kRows - 1) / (2 * kRows);
+  const long long tiles = (long long)g.tiles_t * g.tiles_f;
+  if (tiles > 0x3fffffffll) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: too many tiles for one launch");
+  CUtensorMap tw, tx, tsw, tsx;
+  if (int rc = code_map(&tw, o.w, o.N, o.K, kRows)) return rc;
+  if (int rc = code_map(&tx, o.x, o.M, o.K, kPairTokens / 2)) return rc;
+  if (int rc = scale_map(&tsw, o.sw, o.N, o.K, 1)) return rc;
+  if (int rc = scale_map(&tsx, o.sx, o.M, o.K, 2)) return rc;
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < max_clusters[dev] ? tiles : max_clusters[dev]));
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tw, tx, tsw, tsx, g), "lq_mx_matmul (pair) launch");
+}
+
+template <typename T>
 int launch(const Operands& o, const Args& g, cudaStream_t st) {
+  if (o.M > 128) return launch_pair<T>(o, g, st);
   // the narrowest tile that holds all tokens: the rest of a wider one would be multiplied for nothing
   if (o.M <= 16) return launch_tile<16, T>(o, g, st);
   if (o.M <= 32) return launch_tile<32, T>(o, g, st);

@@ -183,6 +183,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   const int t0 = tile % g.tiles_t * TN, f0 = tile / g.tiles_t * kRows;
   const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
   const int n = kb1 - kb0;
+  const uint32_t smem0 = smem_u32(smem);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * C::kStages + 1; ++s) mbar_init(bar_full + 8 * s, 1);
@@ -202,56 +203,62 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      auto load_w = [&](int i) {
-        const int s = i % C::kStages, kb = kb0 + i;
-        const uint32_t dst = smem_u32(smem + s * C::kStageBytes), bar = bar_full + 8 * s;
-        mbar_expect_tx(bar, C::kStageBytes);
-        tma_load_2d(dst, &tm_w, kb * 128, f0, bar);
-        tma_load_3d(dst + kWBytes + C::kXBytes, &tm_sw, 0, kb, f0 / 128, bar);
-      };
-      // The weight does not depend on the kernel before this one (which encodes the activations): its first
-      // stages are on their way while that one still runs.
-      const int pre = g.early ? min(n, C::kStages) : 0;
-      for (int i = 0; i < pre; ++i) load_w(i);
-      pdl_wait();
-      pdl_launch_dependents();
-      for (int i = 0; i < n; ++i) {
-        const int s = i % C::kStages;
-        if (i >= C::kStages && !mbar_wait(bar_empty + 8 * s, (i / C::kStages - 1) & 1, abort_flag, g.budget)) break;
-        if (i >= pre) load_w(i);
-        const uint32_t dst = smem_u32(smem + s * C::kStageBytes), bar = bar_full + 8 * s;
+    auto load_w = [&](int i, int s) {
+      const uint32_t dst = smem0 + s * C::kStageBytes, bar = bar_full + 8 * s;
+      mbar_expect_tx(bar, C::kStageBytes);
+      tma_load_2d(dst, &tm_w, (kb0 + i) * 128, f0, bar);
+      tma_load_3d(dst + kWBytes + C::kXBytes, &tm_sw, 0, kb0 + i, f0 / mx::kTileRows, bar);
+    };
+    // The weight does not depend on the kernel before this one (which encodes the activations): its first
+    // stages are on their way while that one still runs.
+    const int pre = g.early ? min(n, C::kStages) : 0;
+    for (int i = 0; i < pre; ++i)
+      if (elect_one()) load_w(i, i);
+    pdl_wait();
+    pdl_launch_dependents();
+    int s = 0;
+    uint32_t phase = 1;
+    for (int i = 0; i < n; ++i) {
+      if (!mbar_wait_warp(bar_empty + 8 * s, phase, abort_flag, g.budget)) break;
+      if (elect_one()) {
+        if (i >= pre) load_w(i, s);
+        const uint32_t dst = smem0 + s * C::kStageBytes, bar = bar_full + 8 * s;
         tma_load_2d(dst + kWBytes, &tm_x, (kb0 + i) * 128, t0, bar);
-        tma_load_3d(dst + kWBytes + C::kXBytes + mx::kTileBytes, &tm_sx, 0, kb0 + i, t0 / 128, bar);
+        tma_load_3d(dst + kWBytes + C::kXBytes + mx::kTileBytes, &tm_sx, 0, kb0 + i, t0 / mx::kTileRows, bar);
       }
+      if (++s == C::kStages) s = 0, phase ^= 1;
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int i = 0; i < n; ++i) {
-        const int s = i % C::kStages;
-        if (!mbar_wait(bar_full + 8 * s, (i / C::kStages) & 1, abort_flag, g.budget)) { ok = false; break; }
-        // the scale columns of this buffer were last used two stages ago
-        if (i >= 2 && !mbar_wait(bar_empty + 8 * ((i - 2) % C::kStages), ((i - 2) / C::kStages) & 1, abort_flag, g.budget)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t src = smem_u32(smem + s * C::kStageBytes);
-        const uint32_t ssrc = src + kWBytes + C::kXBytes;
-        const uint32_t sfw = tmem + TN + (i & 1) * 16, sfx = sfw + 8;
+    int s = 0, s2 = C::kStages - 2;  // this stage and the one two before it
+    uint32_t phase = 0, phase2 = 1;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      // the scale columns of this buffer were last used two stages ago
+      if (i >= 2 && !mbar_wait_warp(bar_empty + 8 * s2, phase2, abort_flag, g.budget)) { ok = false; break; }
+      if (!mbar_wait_warp(bar_full + 8 * s, phase, abort_flag, g.budget)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t src = smem0 + s * C::kStageBytes;
+      const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
+      const uint64_t sdesc = scale_desc(src + kWBytes + C::kXBytes);
+      const uint32_t sfw = tmem + TN + (i & 1) * 16, sfx = sfw + 8;
+      if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          tc_cp_scales(sfw + 4 * h, scale_desc(ssrc + h * 512));
-          tc_cp_scales(sfx + 4 * h, scale_desc(ssrc + mx::kTileBytes + h * 512));
+          tc_cp_scales(sfw + 4 * h, sdesc + h * 32);
+          tc_cp_scales(sfx + 4 * h, sdesc + 64 + h * 32);
         }
-        const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           tc_mma_mxf4(tmem, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(kRows, TN, 2 * (k & 1)), sfw + 4 * (k >> 1), sfx + 4 * (k >> 1),
                       i | k ? 1u : 0u);
         tc_commit(bar_empty + 8 * s);
       }
-      if (ok) tc_commit(bar_done);
+      __syncwarp();
+      if (++s == C::kStages) s = 0, phase ^= 1;
+      if (++s2 == C::kStages) s2 = 0, phase2 ^= 1;
     }
+    if (ok && elect_one()) tc_commit(bar_done);
     __syncwarp();
   }
   const bool epilogue = warp >= 2;
@@ -353,6 +360,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   const bool leader = rank == 0;
   const int worker = (int)(blockIdx.x >> 1), workers = (int)(gridDim.x >> 1);
   const int total = g.tiles_t * g.tiles_f;
+  const uint32_t smem0 = smem_u32(smem);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * kPairStages + 2; ++s) mbar_init(bar_full + 8 * s, 1);
@@ -374,60 +382,75 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   pdl_wait();
   pdl_launch_dependents();
 
+  // The issuing warps run their loops with all lanes and elect one for each instruction, with stage and
+  // phase kept as counters: descriptors and loop state then live in uniform registers.  (One lane in a
+  // branch of its own, with the stage taken modulo the ring, cost 820 cycles of issue per stage of 512
+  // cycles of multiplies.)
   if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int tile = worker; ok && tile < total; tile += workers) {
-        const int t0 = tile % g.tiles_t * kPairTokens, f0 = tile / g.tiles_t * 2 * kRows + (int)rank * kRows;
-        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
-          const int s = it % kPairStages;
-          if (it >= kPairStages && !mbar_wait(bar_empty + 8 * s, (it / kPairStages - 1) & 1, abort_flag, g.budget)) { ok = false; break; }
-          const uint32_t dst = smem_u32(smem + s * kPairStageBytes);
+    int s = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (int tile = worker; ok && tile < total; tile += workers) {
+      const int t0 = tile % g.tiles_t * kPairTokens, f0 = tile / g.tiles_t * 2 * kRows + (int)rank * kRows;
+      const int x0 = t0 + (int)rank * (kPairTokens / 2), fr = f0 / mx::kTileRows, tr = t0 / mx::kTileRows;
+      for (int kb = 0; kb < g.num_kb; ++kb) {
+        if (!mbar_wait_warp(bar_empty + 8 * s, phase, abort_flag, g.budget)) { ok = false; break; }
+        const uint32_t dst = smem0 + s * kPairStageBytes;
+        if (elect_one()) {
           const uint32_t full = map_to_cta(bar_full + 8 * s, 0);  // both CTAs' bytes count on the leader's barrier
           if (leader) mbar_expect_tx(bar_full + 8 * s, 2 * kPairStageBytes);
           tma_load_2d_pair(dst, &tm_w, kb * 128, f0, full);
-          tma_load_2d_pair(dst + kWBytes, &tm_x, kb * 128, t0 + (int)rank * (kPairTokens / 2), full);
-          tma_load_3d_pair(dst + kWBytes + kPairXBytes, &tm_sw, 0, kb, f0 / 128, full);
-          tma_load_3d_pair(dst + kWBytes + kPairXBytes + mx::kTileBytes, &tm_sx, 0, kb, t0 / 128, full);
+          tma_load_2d_pair(dst + kWBytes, &tm_x, kb * 128, x0, full);
+          tma_load_3d_pair(dst + kWBytes + kPairXBytes, &tm_sw, 0, kb, fr, full);
+          tma_load_3d_pair(dst + kWBytes + kPairXBytes + mx::kTileBytes, &tm_sx, 0, kb, tr, full);
         }
+        if (++s == kPairStages) s = 0, phase ^= 1;
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (leader && lane == 0) {
-      int it = 0, q = 0;
+    if (leader) {
+      int s = 0, q = 0, done = 0;         // stage; tiles; stages issued (up to 2)
+      int s2 = kPairStages - 2;           // the stage two before this one
+      uint32_t phase = 0, phase2 = 1, buf = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < total; tile += workers, ++q) {
         const int acc = q & 1;
         // this accumulator is empty, and so are the columns it shares with the one before
-        if (q >= 2 && !mbar_wait(bar_tempty + 8 * acc, ((q >> 1) - 1) & 1, abort_flag, g.budget)) break;
-        if (q >= 1 && !mbar_wait(bar_shared, (q - 1) & 1, abort_flag, g.budget)) break;
+        if (q >= 2 && !mbar_wait_warp(bar_tempty + 8 * acc, ((q >> 1) - 1) & 1, abort_flag, g.budget)) break;
+        if (q >= 1 && !mbar_wait_warp(bar_shared, (q - 1) & 1, abort_flag, g.budget)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * kAccStep;
-        for (int kb = 0; kb < g.num_kb; ++kb, ++it) {
-          const int s = it % kPairStages;
-          if (!mbar_wait(bar_full + 8 * s, (it / kPairStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+        for (int kb = 0; kb < g.num_kb; ++kb) {
           // the scale columns of this buffer were last used two stages ago
-          if (it >= 2 && !mbar_wait(bar_empty + 8 * ((it - 2) % kPairStages), ((it - 2) / kPairStages) & 1, abort_flag, g.budget)) { ok = false; break; }
+          if (done == 2 ? !mbar_wait_warp(bar_empty + 8 * s2, phase2, abort_flag, g.budget) : (++done, false)) { ok = false; break; }
+          if (!mbar_wait_warp(bar_full + 8 * s, phase, abort_flag, g.budget)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t src = smem_u32(smem + s * kPairStageBytes);
-          const uint32_t ssrc = src + kWBytes + kPairXBytes;
-          const uint32_t sfw = tmem + kScaleCols + (it & 1) * 24, sfx = sfw + 8;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            tc_cp_scales_pair(sfw + 4 * h, scale_desc(ssrc + h * 512));
-            tc_cp_scales_pair(sfx + 8 * h, scale_desc(ssrc + mx::kTileBytes + h * 512));
-            tc_cp_scales_pair(sfx + 8 * h + 4, scale_desc(ssrc + 2 * mx::kTileBytes + h * 512));
-          }
+          const uint32_t src = smem0 + s * kPairStageBytes;
           const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
+          const uint64_t sdesc = scale_desc(src + kWBytes + kPairXBytes);
+          const uint32_t sfw = tmem + kScaleCols + buf * 24, sfx = sfw + 8;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_mxf4_pair(d, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(2 * kRows, kPairTokens, 2 * (k & 1)), sfw + 4 * (k >> 1),
-                             sfx + 8 * (k >> 1), kb | k ? 1u : 0u);
-          tc_commit_pair(bar_empty + 8 * s);
+            for (int h = 0; h < 2; ++h) {
+              tc_cp_scales_pair(sfw + 4 * h, sdesc + h * 32);
+              tc_cp_scales_pair(sfx + 8 * h, sdesc + 64 + h * 32);
+              tc_cp_scales_pair(sfx + 8 * h + 4, sdesc + 128 + h * 32);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_mxf4_pair(d, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(2 * kRows, kPairTokens, 2 * (k & 1)), sfw + 4 * (k >> 1),
+                               sfx + 8 * (k >> 1), kb | k ? 1u : 0u);
+            tc_commit_pair(bar_empty + 8 * s);
+          }
+          __syncwarp();
+          buf ^= 1;
+          if (++s == kPairStages) s = 0, phase ^= 1;
+          if (++s2 == kPairStages) s2 = 0, phase2 ^= 1;
         }
-        if (ok) tc_commit_pair(bar_tfull + 8 * acc);
+        if (!ok) break;
+        if (elect_one()) tc_commit_pair(bar_tfull + 8 * acc);
+        __syncwarp();
       }
     }
     __syncwarp();

@@ -65,18 +65,6 @@ __device__ __forceinline__ void tc_mma_mxf4_pair(uint32_t d, uint64_t adesc, uin
 __device__ __forceinline__ void tc_cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
-__device__ __forceinline__ void tc_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld_dep8(uint32_t (&r)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-               :
-               : "memory");
-}
 __device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
   asm volatile(
@@ -100,9 +88,9 @@ __device__ __forceinline__ constexpr uint32_t mx_idesc(int m, int n, int id) {
   return ((uint32_t)id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
          ((uint32_t)id << 29);
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
@@ -111,8 +99,26 @@ __device__ __forceinline__ float finish(float v, float bias, bool has_bias, int 
   if (has_bias) v = __fadd_rn(v, bias);
   return relu && v < 0.0f ? 0.0f : v;  // a NaN stays
 }
-__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Four neighbouring features of a token, of which `valid` exist.
+__device__ __forceinline__ void store4(float* p, const float (&v)[4], int valid, int whole) {
+  if (whole && valid >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) p[j] = v[j];
+  }
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4], int valid, int whole) {
+  if (whole && valid >= 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(mx::bf16x2_bits(v[0], v[1]), mx::bf16x2_bits(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) p[j] = __float2bfloat16_rn(v[j]);
+  }
+}
 
 // COUNT tokens [t, t + COUNT) of this lane's feature.  A warp writes 32 neighbouring features of a token per
 // store.  In bf16 two lanes trade halves, so that each writes one word of two features (of the first or
@@ -150,6 +156,7 @@ __device__ __forceinline__ void store_block(const Args& g, const float (&y)[COUN
 // fit an SM, so that the copies of one run during the epilogue of the other.  The partial sums meet in
 // shared memory: every CTA reads the others' through the cluster and adds them in rank order (the same
 // result whatever the timing), each for its share of the outputs.
+constexpr int kMaxSplit = 8;
 constexpr int kThreads = 192;  // producer, multiply, four epilogue warps
 
 template <int TN>
@@ -158,8 +165,8 @@ struct Cfg {
   static constexpr int kStageBytes = kWBytes + kXBytes + 2 * mx::kTileBytes;
   static constexpr int kStages = TN <= 64 ? 4 : 3;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 128;
-  // TMEM: the accumulator, then two buffers of 8 + 8 scale columns (a power of two is allocated)
-  static constexpr int kTmemCols = TN + 32 <= 64 ? 64 : (TN + 32 <= 128 ? 128 : 256);
+  // TMEM: the accumulator, then a buffer of 8 + 8 scale columns per stage (a power of two is allocated)
+  static constexpr int kTmemCols = TN + 16 * kStages <= 128 ? 128 : 256;
   static_assert(2 * kSmemBytes <= 226 * 1024, "two CTAs share an SM");
   static_assert(TN * kRows * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
 };
@@ -230,18 +237,19 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     }
     __syncwarp();
   } else if (warp == 1) {
-    int s = 0, s2 = C::kStages - 2;  // this stage and the one two before it
-    uint32_t phase = 0, phase2 = 1;
+    int s = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      // the scale columns of this buffer were last used two stages ago
-      if (i >= 2 && !mbar_wait_warp(bar_empty + 8 * s2, phase2, abort_flag, g.budget)) { ok = false; break; }
+      // a full stage also says that the multiplies which read its scale columns before are complete: its
+      // copies were issued after them
       if (!mbar_wait_warp(bar_full + 8 * s, phase, abort_flag, g.budget)) { ok = false; break; }
       tc_fence_after();
       const uint32_t src = smem0 + s * C::kStageBytes;
       const uint64_t wdesc = make_smem_desc(src), xdesc = make_smem_desc(src + kWBytes);
       const uint64_t sdesc = scale_desc(src + kWBytes + C::kXBytes);
-      const uint32_t sfw = tmem + TN + (i & 1) * 16, sfx = sfw + 8;
+      // a column holds the scales of 32 rows: a tile of 64 tokens may begin in the middle of a scale tile
+      const uint32_t sfw = tmem + TN + s * 16, sfx = sfw + 8, sft = sfx + (TN < mx::kTileRows ? t0 % mx::kTileRows / 32 : 0);
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -250,13 +258,12 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          tc_mma_mxf4(tmem, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(kRows, TN, 2 * (k & 1)), sfw + 4 * (k >> 1), sfx + 4 * (k >> 1),
+          tc_mma_mxf4(tmem, wdesc + 2 * k, xdesc + 2 * k, mx_idesc(kRows, TN, 2 * (k & 1)), sfw + 4 * (k >> 1), sft + 4 * (k >> 1),
                       i | k ? 1u : 0u);
         tc_commit(bar_empty + 8 * s);
       }
       __syncwarp();
       if (++s == C::kStages) s = 0, phase ^= 1;
-      if (++s2 == C::kStages) s2 = 0, phase2 ^= 1;
     }
     if (ok && elect_one()) tc_commit(bar_done);
     __syncwarp();
@@ -266,7 +273,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   bool ok = true;
   if (epilogue) {
     pdl_wait();
-    ok = mbar_wait_warp<100>(bar_done, 0, abort_flag, g.budget);
+    ok = mbar_wait_warp(bar_done, 0, abort_flag, g.budget);
     tc_fence_after();
   }
   const int valid = min(TN, g.M - t0);
@@ -298,15 +305,24 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     }
     if (!epilogue) pdl_wait();
     cluster_sync_all();
-    const int total = valid * kRows;
+    // four features a step; the loads from all CTAs are issued before the first addition
+    const int total = valid * (kRows / 4);
     const int lo = (int)((long long)total * rank / g.split), hi = (int)((long long)total * (rank + 1) / g.split);
     const uint32_t base = smem_u32(part);
     for (int i = lo + (int)threadIdx.x; i < hi; i += kThreads) {
-      float v = 0.0f;
-      for (int r = 0; r < g.split; ++r) v = __fadd_rn(v, ld_cluster_f32(map_to_cta(base + 4 * i, r)));
-      const int f = f0 + i % kRows, t = t0 + i / kRows;
-      if (f < g.N && *abort_flag == 0)
-        store1(reinterpret_cast<T*>(g.out) + (long long)t * g.ldo + f, finish(v, g.bias ? __ldg(g.bias + f) : 0.0f, g.bias != nullptr, g.relu));
+      float4 p[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < g.split) p[r] = ld_cluster_f32x4(map_to_cta(base + 16 * i, r));
+      const int f = f0 + i % (kRows / 4) * 4, t = t0 + i / (kRows / 4);
+      float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+#pragma unroll
+      for (int r = 1; r < kMaxSplit; ++r)
+        if (r < g.split) v[0] = __fadd_rn(v[0], p[r].x), v[1] = __fadd_rn(v[1], p[r].y), v[2] = __fadd_rn(v[2], p[r].z), v[3] = __fadd_rn(v[3], p[r].w);
+      if (*abort_flag != 0) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = finish(v[j], g.bias && f + j < g.N ? __ldg(g.bias + f + j) : 0.0f, g.bias != nullptr, g.relu);
+      store4(reinterpret_cast<T*>(g.out) + (long long)t * g.ldo + f, v, g.N - f, g.quads_ok);
     }
     cluster_sync_all();  // nobody's partial sums go away while they are read
   }
@@ -328,9 +344,11 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
 // 256 features x 256 tokens per pair of CTAs (cta_group::2): each CTA stages its 128 weight rows and half of
 // the tokens, so a stage of 256 values of K moves 32 KB of codes into each SM for 512 cycles of multiplies --
 // half of what a lone 128 x 128 tile needs, whose operand traffic from L2 is its bound.  TMEM holds two
-// accumulators of 256 columns and two buffers of 24 scale columns only because the accumulators overlap:
-// columns 0..255 and 208..463, scales from 464.  The epilogue empties the 48 shared columns first and
-// says so on a barrier of their own; the next tile's multiplies then run while it works on the rest.
+// accumulators of 256 columns and four buffers of 24 scale columns only because the accumulators overlap:
+// columns 0..255 and 160..415, scales from 416.  The epilogue reads the 96 shared columns into registers
+// first and says so on a barrier of their own; the next tile's multiplies then run while it works on the
+// rest.  (Two scale buffers leave 48 shared columns but make every stage wait for the multiplies two stages
+// back to be reported: 5 % slower.)
 constexpr int kPairTokens = 256;
 constexpr int kPairStages = 6;
 constexpr int kPairXBytes = kPairTokens / 2 * 128;
@@ -338,9 +356,10 @@ constexpr int kPairStageBytes = kWBytes + kPairXBytes + 3 * mx::kTileBytes;
 constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 1024 + 256;
 constexpr int kPairEpilogueWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kPairEpilogueWarps;
-constexpr int kAccStep = 208, kAccShared = kPairTokens - kAccStep;  // columns between the accumulators, and shared
-constexpr int kScaleCols = 464;
-static_assert(kScaleCols >= kAccStep + kPairTokens && kScaleCols + 48 <= 512, "TMEM columns");
+constexpr int kPairScaleBufs = 4;
+constexpr int kScaleCols = 512 - 24 * kPairScaleBufs;
+constexpr int kAccStep = kScaleCols - kPairTokens, kAccShared = kPairTokens - kAccStep;  // columns between the accumulators, and shared
+static_assert(kAccStep % 32 == 0 && kAccShared == 96, "the epilogue's two halves take whole blocks of 16 columns");
 static_assert(kPairSmemBytes <= 227 * 1024, "shared memory");
 
 template <typename T>
@@ -410,9 +429,9 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     __syncwarp();
   } else if (warp == 1) {
     if (leader) {
-      int s = 0, q = 0, done = 0;         // stage; tiles; stages issued (up to 2)
-      int s2 = kPairStages - 2;           // the stage two before this one
-      uint32_t phase = 0, phase2 = 1, buf = 0;
+      int s = 0, q = 0, buf = 0, done = 0;           // stage; tiles; scale buffer; stages issued (up to their number)
+      int sb = kPairStages - kPairScaleBufs;         // the stage that used this scale buffer before
+      uint32_t phase = 0, phase_b = 1;
       bool ok = true;
       for (int tile = worker; ok && tile < total; tile += workers, ++q) {
         const int acc = q & 1;
@@ -422,8 +441,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         tc_fence_after();
         const uint32_t d = tmem + acc * kAccStep;
         for (int kb = 0; kb < g.num_kb; ++kb) {
-          // the scale columns of this buffer were last used two stages ago
-          if (done == 2 ? !mbar_wait_warp(bar_empty + 8 * s2, phase2, abort_flag, g.budget) : (++done, false)) { ok = false; break; }
+          // the multiplies that read this buffer of scale columns before are complete
+          if (done == kPairScaleBufs ? !mbar_wait_warp(bar_empty + 8 * sb, phase_b, abort_flag, g.budget) : (++done, false)) { ok = false; break; }
           if (!mbar_wait_warp(bar_full + 8 * s, phase, abort_flag, g.budget)) { ok = false; break; }
           tc_fence_after();
           const uint32_t src = smem0 + s * kPairStageBytes;
@@ -444,9 +463,9 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
             tc_commit_pair(bar_empty + 8 * s);
           }
           __syncwarp();
-          buf ^= 1;
+          if (++buf == kPairScaleBufs) buf = 0;
           if (++s == kPairStages) s = 0, phase ^= 1;
-          if (++s2 == kPairStages) s2 = 0, phase2 ^= 1;
+          if (++sb == kPairStages) sb = 0, phase_b ^= 1;
         }
         if (!ok) break;
         if (elect_one()) tc_commit_pair(bar_tfull + 8 * acc);
@@ -463,33 +482,35 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
       const int f = tile / g.tiles_t * 2 * kRows + (int)rank * kRows + quad * 32 + lane;
       const int acc = q & 1;
       const float b = g.bias && f < g.N ? __ldg(g.bias + f) : 0.0f;
-      if (!mbar_wait_warp<100>(bar_tfull + 8 * acc, (q >> 1) & 1, abort_flag, g.budget)) break;
+      if (!mbar_wait_warp(bar_tfull + 8 * acc, (q >> 1) & 1, abort_flag, g.budget)) break;
       tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + acc * kAccStep;
-      // [c0, c0 + 8 * blocks) of the tile's tokens, one block of eight read ahead
-      auto drain = [&](int c0, int blocks) {
-        uint32_t r[2][8];
-        tc_ld8(taddr + c0, r[0]);
-#pragma unroll 1
-        for (int i = 0; i < blocks; i += 2) {
+      auto put = [&](const uint32_t (&r)[16], int c) {
+        float y[16];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            if (i + u >= blocks) break;
-            tc_wait_ld_dep8(r[u]);
-            if (i + u + 1 < blocks) tc_ld8(taddr + c0 + 8 * (i + u + 1), r[u ^ 1]);
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = finish(__uint_as_float(r[u][j]), b, g.bias != nullptr, g.relu);
-            if (t0 + c0 + 8 * (i + u) < g.M) store_block<8>(g, y, t0 + c0 + 8 * (i + u), f, lane, (T*)nullptr);
-          }
-        }
+        for (int j = 0; j < 16; ++j) y[j] = finish(__uint_as_float(r[j]), b, g.bias != nullptr, g.relu);
+        if (t0 + c < g.M) store_block<16>(g, y, t0 + c, f, lane, (T*)nullptr);
       };
-      // columns 208..255 of TMEM: the last tokens of the first accumulator, the first of the second
-      drain((acc ? 0 : kAccStep) + half * (kAccShared / 2), kAccShared / 16);
+      // the shared columns of TMEM: the last tokens of the first accumulator, the first of the second
+      const int c_shared = (acc ? 0 : kAccStep) + half * (kAccShared / 2), c_rest = (acc ? kAccShared : 0) + half * (kAccStep / 2);
+      uint32_t r[3][16];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) tc_ld16(taddr + c_shared + 16 * i, r[i]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) tc_wait_ld_dep16(r[i]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(shared_cols);
-      drain((acc ? kAccShared : 0) + half * (kAccStep / 2), kAccStep / 16);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) put(r[i], c_shared + 16 * i);
+      // the rest, one block of 16 columns read ahead
+      tc_ld16(taddr + c_rest, r[0]);
+#pragma unroll
+      for (int i = 0; i < kAccStep / 32; ++i) {
+        tc_wait_ld_dep16(r[i & 1]);
+        if (i + 1 < kAccStep / 32) tc_ld16(taddr + c_rest + 16 * (i + 1), r[(i + 1) & 1]);
+        put(r[i & 1], c_rest + 16 * i);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty + 8 * acc);
@@ -561,7 +582,12 @@ int launch_tile(const Operands& o, Args g, cudaStream_t st) {
   const long long tiles = (long long)g.tiles_t * g.tiles_f;
   const long long room = 2ll * sm_count();
   g.split = 1;
-  while (g.split < 8 && g.split < g.num_kb && tiles * (g.split + 1) <= room) ++g.split;
+  // Share K while all CTAs fit and each keeps enough stages to pay for the exchange of partial sums (which
+  // grows with the tokens).  Measured, split 1 / 2 / 4, us: 256 x 4096 x 4096 (16 stages, 64 tokens a tile)
+  // 8.2 / 9.3 / 9.3; 48 x 8192 x 10240 (32 stages) 14.4 / 13.7 / 12.0; 1 x 8192 x 8192 12.0 / 9.8 / 9.0;
+  // 1 x 1024 x 8192 (4 stages) 2.9 / 3.3 / 4.2.
+  const int least = TN <= 32 ? 4 : 10;
+  while (g.split < kMaxSplit && g.num_kb >= least * (g.split + 1) && tiles * (g.split + 1) <= room) ++g.split;
   if (tiles * g.split > 0x7fffffffll) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: too many tiles for one launch");
   CUtensorMap tw, tx, tsw, tsx;
   if (int rc = code_map(&tw, o.w, o.N, o.K, kRows)) return rc;
@@ -617,12 +643,16 @@ int launch_pair(const Operands& o, Args g, cudaStream_t st) {
 
 template <typename T>
 int launch(const Operands& o, const Args& g, cudaStream_t st) {
-  if (o.M > 128) return launch_pair<T>(o, g, st);
-  // the narrowest tile that holds all tokens: the rest of a wider one would be multiplied for nothing
+  // Up to 64 tokens: the narrowest tile that holds them all (the weight's stream is the bound, the rest of
+  // a wider tile would be multiplied for nothing).  More: the narrowest tile whose count fits the GPU at
+  // once, two CTAs an SM, and pairs beyond that.  Measured, tile of 64 / 128 tokens / pair, us: 256 x 4096 x
+  // 4096 8.2 / 10.1 / 13.7; 1000 x 4096 x 4096 17.9 / 12.2 / 14.4; 2048 x 4096 x 4096 34.0 / 24.4 / 22.5.
   if (o.M <= 16) return launch_tile<16, T>(o, g, st);
   if (o.M <= 32) return launch_tile<32, T>(o, g, st);
-  if (o.M <= 64) return launch_tile<64, T>(o, g, st);
-  return launch_tile<128, T>(o, g, st);
+  const long long rows = (long long)((o.N + kRows - 1) / kRows), room = 2ll * sm_count();
+  if (o.M <= 64 || (long long)((o.M + 63) / 64) * rows <= room) return launch_tile<64, T>(o, g, st);
+  if ((long long)((o.M + 127) / 128) * rows <= room) return launch_tile<128, T>(o, g, st);
+  return launch_pair<T>(o, g, st);
 }
 
 int matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes, const uint8_t* w_scales, size_t N, size_t K,
@@ -642,6 +672,7 @@ int matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint
   g.M = (int)M, g.N = (int)N, g.num_kb = (int)((K + kStageK - 1) / kStageK);
   g.early = early, g.bias = bias, g.relu = relu, g.out = out, g.ldo = (long long)ldo, g.status = status, g.budget = kWaitBudgetCycles;
   g.pairs_ok = out_dtype == LQ_BF16 && reinterpret_cast<uintptr_t>(out) % 4 == 0 && ldo % 2 == 0 && N % 2 == 0;
+  g.quads_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
   const Operands o = {a_codes, a_scales, w_codes, w_scales, M, N, K};
   return out_dtype == LQ_F32 ? launch<float>(o, g, st) : launch<__nv_bfloat16>(o, g, st);
 }

@@ -259,12 +259,17 @@ def stream_ptr(device=None):
 def call(name: str, device: torch.device, *args) -> None:
     """One library call on ``device`` and its current stream (which is the entry's last argument),
     its status checked."""
-    fn = getattr(load(), name)
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    fn = getattr(_lib or load(), name)
+    index = device.index
+    # the raw handle: a Stream object costs 2 us a call, as much as the launch itself
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(*args, stream)
+    if rc:
+        check(rc)
 
 
 # per-(device, stream) zero-initialised workspace for the per-tensor range reduction

@@ -171,59 +171,114 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
 
 // ---- read ----------------------------------------------------------------------------------------------
 
-template <typename T, bool MXF>
-__global__ void __launch_bounds__(kThreads)
-kv_read_kernel(const Side k, const Side v, long long n_pages, int page, int heads, int dim, const int* __restrict__ table,
-               long long table_stride, int max_blocks, const int* __restrict__ cu, const int* __restrict__ starts, int seqs,
-               size_t total, int clear_tail, int32_t* status) {
-  const size_t r = ((size_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-  if (r >= total) return;
-  const int lane = threadIdx.x & 31;
-  // the sequence whose rows [cu[b], cu[b + 1]) hold r
-  int lo = 0, hi = seqs;  // first index in [0, seqs] with cu[index] > r
-  bool covered = (long long)r < (long long)__ldg(cu + seqs) && (long long)r >= (long long)__ldg(cu);
-  if (!covered && !clear_tail) return;
+// n / d for n * d < 2^40, by a multiplication
+struct FastDiv {
+  uint32_t d;
+  unsigned long long m;  // ceil(2^40 / d)
+  __host__ explicit FastDiv(uint32_t div) : d(div), m((((unsigned long long)1 << 40) + div - 1) / div) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 40); }
+};
+
+struct Table {
+  const int* pages;
+  long long stride;
+  int max_blocks;
+  const int* cu;
+  const int* starts;
+  int seqs;
+  long long n_pages;
+  int page;
+};
+
+// Slot of output row r, -1 where the table has none for it; `covered` says whether a sequence has the row.
+__device__ __forceinline__ long long find_slot(const Table& t, long long r, bool& covered) {
+  covered = r < (long long)__ldg(t.cu + t.seqs) && r >= (long long)__ldg(t.cu);
+  if (!covered) return -1;
+  int lo = 0, hi = t.seqs;  // the first index with cu[index] > r
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if ((long long)__ldg(cu + mid) > (long long)r) hi = mid;
+    if ((long long)__ldg(t.cu + mid) > r) hi = mid;
     else lo = mid + 1;
   }
-  long long slot = -1;
-  if (covered && lo > 0) {
-    const int b = lo - 1;
-    const long long pos = (long long)r - __ldg(cu + b) + (starts ? __ldg(starts + b) : 0);
-    const long long blk = pos / page;
-    if (pos >= 0 && blk < max_blocks) {
-      const long long p = __ldg(table + b * table_stride + blk);
-      if (p >= 0 && p < n_pages) slot = p * page + pos % page;
-    }
-    if (slot < 0 && status && lane == 0) atomicExch(status, (int)LQ_ERR_SHAPE);
+  if (lo == 0) return -1;  // cu does not ascend
+  const int b = lo - 1;
+  const long long pos = r - __ldg(t.cu + b) + (t.starts ? __ldg(t.starts + b) : 0);
+  if (pos < 0 || pos > 0x7fffffffll) return -1;
+  const int blk = (int)pos / t.page;
+  if (blk >= t.max_blocks) return -1;
+  const long long p = __ldg(t.pages + b * t.stride + blk);
+  return p < 0 || p >= t.n_pages ? -1 : p * t.page + (int)pos % t.page;
+}
+
+// A warp reads TOKENS consecutive output rows.  Its lanes first look up one row each (the search through
+// cu_seqlens and the page table is a chain of dependent loads, so it is walked for all rows at once), then
+// walk the rows' values together, 16 of a head per lane and step, four steps' loads in flight.  Bound by HBM:
+// a byte (half a byte) read and two or four written per value.
+template <typename T, bool MXF, int TOKENS>
+__global__ void __launch_bounds__(kThreads)
+kv_read_kernel(const Side k, const Side v, const Table t, int heads, const FastDiv per_row, const FastDiv per_side,
+               const FastDiv per_head, long long total, int clear_tail, int wide, int32_t* status) {
+  const long long r0 = (((long long)blockIdx.x * kThreads + threadIdx.x) >> 5) * TOKENS;
+  if (r0 >= total) return;
+  const int lane = threadIdx.x & 31;
+  const int rows = (int)(total - r0 < TOKENS ? total - r0 : TOKENS);
+  long long slot = -2;  // -2: left alone, -1: zeros
+  if (lane < rows) {
+    bool covered;
+    slot = find_slot(t, r0 + lane, covered);
+    if (slot < 0 && covered && status) atomicExch(status, (int)LQ_ERR_SHAPE);
+    if (!covered) slot = clear_tail ? -1 : -2;
   }
-  const int per_head = dim / 8;
-  for (int c = lane; c < heads * per_head * 2; c += 32) {
-    const int side = c / (heads * per_head), cc = c - side * heads * per_head;
-    const int head = cc / per_head, d0 = (cc - head * per_head) * 8;
-    const Side& sd = side ? v : k;
-    float f[8];
-    if (slot < 0) {
+  const uint32_t chunks = rows * per_row.d;  // 16 values each: row, keys or values, head, place in the head
+  const int dim = (int)per_head.d * 16;
+  constexpr int kSteps = 4;
+  for (uint32_t c0 = 0; c0 < chunks; c0 += 32 * kSteps) {
+    uint4 code[kSteps];
+    float scale[kSteps];
+    T* dst[kSteps];
+    long long at[kSteps];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.0f;
-    } else {
-      const size_t row = (size_t)slot * heads + head;
-      float s;
-      if (MXF) {
-        mx::decode8(__ldg(reinterpret_cast<const uint32_t*>(sd.codes + row * (dim / 2) + d0 / 2)), f);
-        s = mx::scale_value(__ldg(sd.scales + row * (dim / 32) + d0 / 32));
+    for (int u = 0; u < kSteps; ++u) {
+      const uint32_t c = c0 + u * 32 + lane;
+      const uint32_t i = per_row(c);
+      at[u] = __shfl_sync(0xffffffffu, slot, i < TOKENS ? i : 0);
+      if (c >= chunks) at[u] = -2;
+      const uint32_t w = c - i * per_row.d, side = per_side(w), x = w - side * per_side.d;
+      const uint32_t head = per_head(x), d0 = (x - head * per_head.d) * 16;
+      const Side& sd = side ? v : k;
+      dst[u] = reinterpret_cast<T*>(sd.out) + (r0 + i) * sd.out_token + head * sd.out_head + d0;
+      if (at[u] >= 0) {
+        const size_t row = (size_t)at[u] * heads + head;
+        if (MXF) {
+          const uint2 q = __ldg(reinterpret_cast<const uint2*>(sd.codes + row * (dim / 2) + d0 / 2));
+          code[u] = make_uint4(q.x, q.y, 0, 0);
+          scale[u] = mx::scale_value(__ldg(sd.scales + row * (dim / 32) + d0 / 32));
+        } else {
+          code[u] = ld_stream_u4(sd.codes + row * dim + d0);
+          scale[u] = __ldg(reinterpret_cast<const float*>(sd.scales) + row);
+        }
       } else {
-        const int2 w = __ldg(reinterpret_cast<const int2*>(sd.codes + row * dim + d0));
+        code[u] = make_uint4(0, 0, 0, 0), scale[u] = 0.0f;
+      }
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w.x >> (8 * i)), f[4 + i] = (float)(int8_t)(w.y >> (8 * i));
-        s = __ldg(reinterpret_cast<const float*>(sd.scales) + row);
+    for (int u = 0; u < kSteps; ++u) {
+      if (at[u] == -2) continue;
+      float lo[8], hi[8];
+      if (MXF) {
+        mx::decode8(code[u].x, lo);
+        mx::decode8(code[u].y, hi);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = (float)(int8_t)(code[u].x >> (8 * j)), lo[4 + j] = (float)(int8_t)(code[u].y >> (8 * j));
+          hi[j] = (float)(int8_t)(code[u].z >> (8 * j)), hi[4 + j] = (float)(int8_t)(code[u].w >> (8 * j));
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], s);
+      for (int j = 0; j < 8; ++j) lo[j] = __fmul_rn(lo[j], scale[u]), hi[j] = __fmul_rn(hi[j], scale[u]);
+      mx::store16(dst[u], lo, hi, wide);
     }
-    mx::store8(reinterpret_cast<T*>(sd.out) + (long long)r * sd.out_token + head * sd.out_head + d0, f);
   }
 }
 
@@ -305,19 +360,32 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_read: the cache must be 16-byte aligned");
   Side ks = {nullptr, 0, 0, (uint8_t*)k_codes, (uint8_t*)k_scales, out_k, (long long)k_token, (long long)k_head};
   Side vs = {nullptr, 0, 0, (uint8_t*)v_codes, (uint8_t*)v_scales, out_v, (long long)v_token, (long long)v_head};
-  const unsigned grid = (unsigned)((total * 32 + kThreads - 1) / kThreads);
+  const Table t = {table, (long long)table_stride, (int)max_blocks, cu_seqlens, starts, (int)seqs, (long long)n_pages, (int)page};
+  const uint32_t head_chunks = (uint32_t)(dim / 16), side_chunks = head_chunks * (uint32_t)heads;
+  const int wide = ((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) % 32 == 0) &&
+                   ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
+  // four rows a warp once that still gives every SM a few dozen warps; one row below
+  const bool few = total < 4 * 32 * (size_t)sm_count();
+  const size_t warps = few ? total : (total + 3) / 4;
+  const unsigned grid = (unsigned)((warps * 32 + kThreads - 1) / kThreads);
   cudaStream_t st = (cudaStream_t)stream;
-#define LQ_KV_READ(T, F)                                                                                                        \
-  kv_read_kernel<T, F><<<grid, kThreads, 0, st>>>(ks, vs, (long long)n_pages, (int)page, (int)heads, (int)dim, table,            \
-                                                  (long long)table_stride, (int)max_blocks, cu_seqlens, starts, (int)seqs, total, \
-                                                  clear_tail, status)
-  if (out_dtype == LQ_F32) {
-    if (format == LQ_KV_MXFP4) LQ_KV_READ(float, true);
-    else LQ_KV_READ(float, false);
-  } else {
-    if (format == LQ_KV_MXFP4) LQ_KV_READ(bf16, true);
-    else LQ_KV_READ(bf16, false);
+#define LQ_KV_READ(T, F, N)                                                                                              \
+  kv_read_kernel<T, F, N><<<grid, kThreads, 0, st>>>(ks, vs, t, (int)heads, FastDiv(2 * side_chunks), FastDiv(side_chunks), \
+                                                     FastDiv(head_chunks), (long long)total, clear_tail, wide, status)
+#define LQ_KV_READ_T(T)                                     \
+  if (format == LQ_KV_MXFP4) {                              \
+    if (few) LQ_KV_READ(T, true, 1);                        \
+    else LQ_KV_READ(T, true, 4);                            \
+  } else {                                                  \
+    if (few) LQ_KV_READ(T, false, 1);                       \
+    else LQ_KV_READ(T, false, 4);                           \
   }
+  if (out_dtype == LQ_F32) {
+    LQ_KV_READ_T(float)
+  } else {
+    LQ_KV_READ_T(bf16)
+  }
+#undef LQ_KV_READ_T
 #undef LQ_KV_READ
   return check_cuda(cudaGetLastError(), "lq_kv_read launch");
 }

@@ -89,6 +89,12 @@ struct Chunk<float> {
   __device__ __forceinline__ void load(const float* p) {
     a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
   }
+  // one 32-byte load: p is 32-byte aligned
+  __device__ __forceinline__ void load_wide(const float* p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(p));
+  }
   __device__ __forceinline__ void clear() { a = b = make_uint4(0, 0, 0, 0); }
   // float32 bit pattern of the largest magnitude (ordered like the magnitudes, NaN above infinity)
   __device__ __forceinline__ uint32_t amax_bits() const {
@@ -108,7 +114,8 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 template <>
 struct Chunk<__nv_bfloat16> {
   uint4 a;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = ld_stream_u4(p); }
+  __device__ __forceinline__ void load_wide(const __nv_bfloat16* p) { load(p); }
   __device__ __forceinline__ void clear() { a = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ uint32_t amax_bits() const {
     const uint32_t m = 0x7fff7fffu;
@@ -127,6 +134,11 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
+__device__ __forceinline__ void store_32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -134,6 +146,34 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) =
       make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7]));
+}
+
+// ... in one store per 32 bytes where the address allows it (`wide`)
+__device__ __forceinline__ void store8(float* p, const float (&v)[8], int wide) {
+  if (wide) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+    store_32(p, w);
+  } else {
+    store8(p, v);
+  }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8], int) { store8(p, v); }
+// Sixteen values.
+__device__ __forceinline__ void store16(float* p, const float (&lo)[8], const float (&hi)[8], int wide) {
+  store8(p, lo, wide);
+  store8(p + 8, hi, wide);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&lo)[8], const float (&hi)[8], int wide) {
+  if (wide) {
+    const uint32_t w[8] = {bf16x2_bits(lo[0], lo[1]), bf16x2_bits(lo[2], lo[3]), bf16x2_bits(lo[4], lo[5]), bf16x2_bits(lo[6], lo[7]),
+                           bf16x2_bits(hi[0], hi[1]), bf16x2_bits(hi[2], hi[3]), bf16x2_bits(hi[4], hi[5]), bf16x2_bits(hi[6], hi[7])};
+    store_32(p, w);
+  } else {
+    store8(p, lo);
+    store8(p + 8, hi);
+  }
 }
 
 }  // namespace mx

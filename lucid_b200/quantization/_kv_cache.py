@@ -47,35 +47,36 @@ def kv_cache_alloc(num_pages: int, page_size: int, heads: int, head_dim: int, fm
 
 
 def _check_cache(cache) -> tuple:
-    """``(format, pages, page_size, heads, dim)`` of a cache whose tensors agree with each other."""
+    """``(format, pages, page_size, heads, dim, device)`` of a cache whose tensors agree with each other."""
     kc, ks, vc, vs = cache
     _lib.require_cuda(kc, "cache k_codes")
-    if kc.dim() != 4:
-        raise _lib.ShapeMismatch(f"cache codes must be (pages, page_size, heads, ..), got {tuple(kc.shape)}")
+    shape = kc.shape
+    if len(shape) != 4:
+        raise _lib.ShapeMismatch(f"cache codes must be (pages, page_size, heads, ..), got {tuple(shape)}")
+    pages, page, heads, width = shape
     if kc.dtype == torch.int8:
-        fmt, dim, scale_dtype, scale_shape = _lib.KV_INT8, kc.shape[3], torch.float32, kc.shape[:3]
+        fmt, dim, scale_dtype, scale_shape = _lib.KV_INT8, width, torch.float32, shape[:3]
     elif kc.dtype == torch.uint8:
-        fmt, dim, scale_dtype = _lib.KV_MXFP4, kc.shape[3] * 2, torch.uint8
-        scale_shape = (*kc.shape[:3], kc.shape[3] // 16)
+        fmt, dim, scale_dtype, scale_shape = _lib.KV_MXFP4, width * 2, torch.uint8, (pages, page, heads, width // 16)
     else:
         raise _lib.DtypeMismatch(f"cache codes must be int8 or uint8 (MXFP4), got {kc.dtype}")
-    for name, t, dtype, shape in (("k_scales", ks, scale_dtype, scale_shape), ("v_codes", vc, kc.dtype, kc.shape),
-                                  ("v_scales", vs, scale_dtype, scale_shape)):
-        if not isinstance(t, torch.Tensor) or t.device != kc.device:
-            raise _lib.DeviceMismatch(f"cache {name} must be a tensor on {kc.device}")
-        if t.dtype != dtype:
-            raise _lib.DtypeMismatch(f"cache {name} must be {dtype}, got {t.dtype}")
-        if t.shape != shape:
-            raise _lib.ShapeMismatch(f"cache {name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    dev = kc.device
+    if not (ks.device == dev and vc.device == dev and vs.device == dev):
+        raise _lib.DeviceMismatch(f"the tensors of a cache must be on one device, got {[str(t.device) for t in cache]}")
+    if ks.dtype != scale_dtype or vc.dtype != kc.dtype or vs.dtype != scale_dtype:
+        raise _lib.DtypeMismatch(f"cache of {kc.dtype} codes: expected {scale_dtype} scales, got {[t.dtype for t in cache]}")
+    if ks.shape != scale_shape or vc.shape != shape or vs.shape != scale_shape:
+        raise _lib.ShapeMismatch(f"codes {tuple(shape)} go with scales {tuple(scale_shape)}, got {[tuple(t.shape) for t in cache]}")
     if not (kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
         raise _lib.ShapeMismatch("the tensors of a cache must be contiguous")
-    return fmt, kc.shape[0], kc.shape[1], kc.shape[2], dim
+    return fmt, pages, page, heads, dim, dev
 
 
 def _row_view(t: torch.Tensor) -> bool:
     """Whether the kernel can walk ``(tokens, heads, dim)`` as it lies: contiguous dim, 16-byte rows."""
+    sn, sh, one = t.stride()
     step = 16 // t.element_size()
-    return t.stride(2) == 1 and t.stride(0) % step == 0 and t.stride(1) % step == 0 and t.data_ptr() % 16 == 0
+    return one == 1 and sn % step == 0 and sh % step == 0 and t.data_ptr() % 16 == 0
 
 
 def _distinct_rows(t: torch.Tensor) -> bool:
@@ -93,33 +94,29 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     status word (``lucid_b200._lib.check_device_status``); nothing is synchronised here.  When a slot
     occurs twice the later token stays.  A row that holds a NaN or an infinity reads back as NaN (in
     MXFP4: its blocks of 32 that do)."""
-    fmt, pages, page, heads, dim = _check_cache(cache)
-    dev = cache.k_codes.device
-    for name, t in (("k", k), ("v", v)):
-        _lib.require_cuda(t, name)
-        if t.device != dev:
-            raise _lib.DeviceMismatch(f"{name} on {t.device}, the cache on {dev}")
-        if t.dtype not in _FLOATS:
-            raise _lib.DtypeMismatch(f"{name} must be float32 or bfloat16, got {t.dtype}")
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-            raise _lib.ShapeMismatch(f"{name} is {tuple(t.shape)}, expected (tokens, {heads}, {dim})")
-    if k.dtype != v.dtype:
-        raise _lib.DtypeMismatch(f"k is {k.dtype}, v {v.dtype}")
+    fmt, pages, page, heads, dim, dev = _check_cache(cache)
+    _lib.require_cuda(k, "k")
+    _lib.require_cuda(v, "v")
     _lib.require_cuda(slots, "slots")
-    if slots.device != dev:
-        raise _lib.DeviceMismatch(f"slots on {slots.device}, the cache on {dev}")
-    if slots.dtype not in (torch.int32, torch.int64):
+    if k.device != dev or v.device != dev or slots.device != dev:
+        raise _lib.DeviceMismatch(f"k on {k.device}, v on {v.device}, slots on {slots.device}, the cache on {dev}")
+    if k.dtype not in _FLOATS or v.dtype != k.dtype:
+        raise _lib.DtypeMismatch(f"k and v must both be float32 or both bfloat16, got {k.dtype}, {v.dtype}")
+    if slots.dtype != torch.int64 and slots.dtype != torch.int32:
         raise _lib.DtypeMismatch(f"slots must be int32 or int64, got {slots.dtype}")
-    tokens = k.shape[0]
-    if v.shape[0] != tokens or tuple(slots.shape) != (tokens,):
-        raise _lib.ShapeMismatch(f"{tokens} rows of k, {v.shape[0]} of v, slots {tuple(slots.shape)}")
-    k, v = k.detach(), v.detach()
-    k = k if _row_view(k) else k.clone(memory_format=torch.contiguous_format)
-    v = v if _row_view(v) else v.clone(memory_format=torch.contiguous_format)
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape or slots.shape != shape[:1]:
+        raise _lib.ShapeMismatch(f"expected k and v (tokens, {heads}, {dim}) and slots (tokens,), got {tuple(shape)}, "
+                                 f"{tuple(v.shape)}, {tuple(slots.shape)}")
+    k = k if _row_view(k) else k.detach().clone(memory_format=torch.contiguous_format)
+    v = v if _row_view(v) else v.detach().clone(memory_format=torch.contiguous_format)
     slots = slots.contiguous()
-    _lib.call("lq_kv_write", dev, k.data_ptr(), v.data_ptr(), _lib.code_of(k.dtype), tokens, heads, dim, k.stride(0), k.stride(1),
-          v.stride(0), v.stride(1), slots.data_ptr(), 64 if slots.dtype == torch.int64 else 32, pages * page, fmt,
-          *(t.data_ptr() for t in cache), _lib.status_word(dev).data_ptr())
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    kc, ks, vc, vs = cache
+    _lib.call("lq_kv_write", dev, k.data_ptr(), v.data_ptr(), _lib.code_of(k.dtype), shape[0], heads, dim, kt, kh, vt, vh,
+              slots.data_ptr(), 64 if slots.dtype == torch.int64 else 32, pages * page, fmt, kc.data_ptr(), ks.data_ptr(),
+              vc.data_ptr(), vs.data_ptr(), _lib.status_word(dev).data_ptr())
 
 
 def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -133,33 +130,38 @@ def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.
     tensors of any token and head stride; rows that no sequence covers keep what they held there,
     and are zeros in tensors allocated here.  A token past its row of the table, or a page outside
     the cache, reads as zeros and sets the device status word."""
-    fmt, pages, page, heads, dim = _check_cache(cache)
-    dev = cache.k_codes.device
-    for name, t, dims in (("block_tables", block_tables, 2), ("cu_seqlens", cu_seqlens, 1), ("starts", starts, 1)):
-        if t is None:
-            continue
-        _lib.require_cuda(t, name)
-        if t.device != dev:
-            raise _lib.DeviceMismatch(f"{name} on {t.device}, the cache on {dev}")
-        if t.dtype != torch.int32:
-            raise _lib.DtypeMismatch(f"{name} must be int32, got {t.dtype}")
-        if t.dim() != dims:
-            raise _lib.ShapeMismatch(f"{name} must have {dims} axes, got {tuple(t.shape)}")
+    fmt, pages, page, heads, dim, dev = _check_cache(cache)
+    _lib.require_cuda(block_tables, "block_tables")
+    _lib.require_cuda(cu_seqlens, "cu_seqlens")
+    if block_tables.device != dev or cu_seqlens.device != dev:
+        raise _lib.DeviceMismatch(f"block_tables on {block_tables.device}, cu_seqlens on {cu_seqlens.device}, the cache on {dev}")
+    if block_tables.dtype != torch.int32 or cu_seqlens.dtype != torch.int32:
+        raise _lib.DtypeMismatch(f"block_tables and cu_seqlens must be int32, got {block_tables.dtype}, {cu_seqlens.dtype}")
+    if block_tables.dim() != 2:
+        raise _lib.ShapeMismatch(f"block_tables must be (sequences, max_pages), got {tuple(block_tables.shape)}")
     seqs, max_blocks = block_tables.shape
-    if cu_seqlens.shape[0] != seqs + 1 or (starts is not None and starts.shape[0] != seqs):
-        raise _lib.ShapeMismatch(f"{seqs} rows of block_tables, cu_seqlens {tuple(cu_seqlens.shape)}"
-                                 + ("" if starts is None else f", starts {tuple(starts.shape)}"))
+    if cu_seqlens.shape != (seqs + 1,):
+        raise _lib.ShapeMismatch(f"{seqs} rows of block_tables need {seqs + 1} cu_seqlens, got {tuple(cu_seqlens.shape)}")
+    if starts is not None:
+        _lib.require_cuda(starts, "starts")
+        if starts.device != dev:
+            raise _lib.DeviceMismatch(f"starts on {starts.device}, the cache on {dev}")
+        if starts.dtype != torch.int32:
+            raise _lib.DtypeMismatch(f"starts must be int32, got {starts.dtype}")
+        if starts.shape != (seqs,):
+            raise _lib.ShapeMismatch(f"{seqs} sequences, starts {tuple(starts.shape)}")
+        starts = starts.contiguous()
     total = int(total)
     if total < 0 or total >= 1 << 31:
         raise _lib.ShapeMismatch(f"total must be in [0, 2^31), got {total}")
-    shape = (total, heads, dim)
     if out is None:
         if out_dtype not in _FLOATS:
             raise _lib.DtypeMismatch(f"kv_cache_read writes float32 or bfloat16, got {out_dtype}")
-        ok = torch.empty(shape, dtype=out_dtype, device=dev)
-        ov = torch.empty(shape, dtype=out_dtype, device=dev)
+        ok = torch.empty(total, heads, dim, dtype=out_dtype, device=dev)
+        ov = torch.empty(total, heads, dim, dtype=out_dtype, device=dev)
     else:
         ok, ov = out
+        shape = (total, heads, dim)
         for t in (ok, ov):
             if not isinstance(t, torch.Tensor) or t.device != dev:
                 raise _lib.DeviceMismatch(f"out= must be tensors on {dev}")
@@ -171,8 +173,10 @@ def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.
                 raise _lib.ShapeMismatch("out= needs a contiguous last axis and 16-byte aligned rows that do not overlap")
     table = block_tables if max_blocks <= 1 or block_tables.stride(1) == 1 else block_tables.contiguous()
     cu = cu_seqlens.contiguous()
-    st = None if starts is None else starts.contiguous()
-    _lib.call("lq_kv_read", dev, *(t.data_ptr() for t in cache), fmt, pages, page, heads, dim, table.data_ptr(), table.stride(0),
-          max_blocks, cu.data_ptr(), _addr(st), seqs, total, ok.data_ptr(), ov.data_ptr(), _lib.code_of(ok.dtype),
-          ok.stride(0), ok.stride(1), ov.stride(0), ov.stride(1), int(out is None), _lib.status_word(dev).data_ptr())
+    kt, kh, _ = ok.stride()
+    vt, vh, _ = ov.stride()
+    kc, ks, vc, vs = cache
+    _lib.call("lq_kv_read", dev, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), fmt, pages, page, heads, dim,
+              table.data_ptr(), table.stride(0), max_blocks, cu.data_ptr(), _addr(starts), seqs, total, ok.data_ptr(),
+              ov.data_ptr(), _lib.code_of(ok.dtype), kt, kh, vt, vh, int(out is None), _lib.status_word(dev).data_ptr())
     return ok, ov

@@ -27,18 +27,23 @@ def _float_input(x, what: str) -> torch.Tensor:
     _lib.require_cuda(x, what)
     if x.dtype not in _FLOATS:
         raise _lib.DtypeMismatch(f"{what} must be float32 or bfloat16, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 32 != 0:
-        raise _lib.ShapeMismatch(f"{what} needs a last axis that is a multiple of 32, got {tuple(x.shape)}")
-    return x.detach()
+    shape = x.shape
+    if not shape or shape[-1] == 0 or shape[-1] % 32:
+        raise _lib.ShapeMismatch(f"{what} needs a last axis that is a multiple of 32, got {tuple(shape)}")
+    return x.detach() if x.requires_grad else x
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as (rows, K) with unit column stride and 16-byte aligned rows, copied only if it has to be."""
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    step = 16 // x2.element_size()
-    if x2.stride(1) != 1 or x2.stride(0) % step or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2
+def _rows(x: torch.Tensor) -> tuple:
+    """``(x2, rows, K, row stride)``: ``x`` as (rows, K) with unit column stride and 16-byte aligned rows,
+    copied only if it has to be."""
+    k = x.shape[-1]
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, x.numel() // k, k, k
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    ld, one = x2.stride()
+    if one != 1 or ld * x2.element_size() % 16 or ld < k or x2.data_ptr() % 16:
+        x2, ld = x2.clone(memory_format=torch.contiguous_format), k
+    return x2, x2.shape[0], k, ld
 
 
 def _dense(x: torch.Tensor) -> torch.Tensor:
@@ -52,17 +57,18 @@ def _scale_shape(rows: int, k: int) -> tuple:
 
 def _check_packed(codes, scales, what: str) -> tuple:
     """``(codes, scales, rows, K)`` of a packed matrix, its two tensors checked against each other."""
-    for t, name in ((codes, "codes"), (scales, "scales")):
-        _lib.require_cuda(t, f"{what} {name}")
-        if t.dtype != torch.uint8:
-            raise _lib.DtypeMismatch(f"{what} {name} must be uint8, got {t.dtype}")
+    _lib.require_cuda(codes, what)
+    _lib.require_cuda(scales, what)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise _lib.DtypeMismatch(f"{what}: codes and scales must be uint8, got {codes.dtype}, {scales.dtype}")
     if scales.device != codes.device:
         raise _lib.DeviceMismatch(f"{what}: codes on {codes.device}, scales on {scales.device}")
-    if codes.dim() == 0 or codes.shape[-1] == 0 or codes.shape[-1] % 16 != 0:
-        raise _lib.ShapeMismatch(f"{what} codes need a last axis that is a multiple of 16, got {tuple(codes.shape)}")
-    k = codes.shape[-1] * 2
-    rows = codes.numel() * 2 // k
-    if tuple(scales.shape) != _scale_shape(rows, k):
+    shape = codes.shape
+    if not shape or shape[-1] == 0 or shape[-1] % 16:
+        raise _lib.ShapeMismatch(f"{what} codes need a last axis that is a multiple of 16, got {tuple(shape)}")
+    k = shape[-1] * 2
+    rows = shape[0] if len(shape) == 2 else codes.numel() * 2 // k
+    if scales.shape != _scale_shape(rows, k):
         raise _lib.ShapeMismatch(f"{what} scales are {tuple(scales.shape)}, expected {_scale_shape(rows, k)}")
     return _dense(codes), _dense(scales), rows, k
 
@@ -71,12 +77,11 @@ def mx_quantize(x: torch.Tensor):
     """``(codes, scales)`` of ``x`` (float32 or bfloat16, the last axis a multiple of 32).  A block with
     a NaN or an infinity decodes to NaN."""
     x = _float_input(x, "mx_quantize input")
-    x2 = _rows(x)
-    rows, k = x2.shape
-    codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_shape(rows, k), dtype=torch.uint8, device=x.device)
-    _lib.call("lq_mx_quantize", x.device, x2.data_ptr(), _lib.code_of(x2.dtype), rows, k, x2.stride(0), codes.data_ptr(),
-          scales.data_ptr())
+    x2, rows, k, ld = _rows(x)
+    dev = x.device
+    codes = torch.empty(*x.shape[:-1], k // 2, dtype=torch.uint8, device=dev)
+    scales = torch.empty(*_scale_shape(rows, k), dtype=torch.uint8, device=dev)
+    _lib.call("lq_mx_quantize", dev, x2.data_ptr(), _lib.code_of(x.dtype), rows, k, ld, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -85,8 +90,17 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dt
     if out_dtype not in _FLOATS:
         raise _lib.DtypeMismatch(f"mx_dequantize writes float32 or bfloat16, got {out_dtype}")
     c, s, rows, k = _check_packed(codes, scales, "mx_dequantize")
-    out = torch.empty((*codes.shape[:-1], k), dtype=out_dtype, device=codes.device)
-    _lib.call("lq_mx_dequantize", codes.device, c.data_ptr(), s.data_ptr(), rows, k, out.data_ptr(), _lib.code_of(out_dtype))
+    dev = codes.device
+    out = torch.empty(*codes.shape[:-1], k, dtype=out_dtype, device=dev)
+    _lib.call("lq_mx_dequantize", dev, c.data_ptr(), s.data_ptr(), rows, k, out.data_ptr(), _lib.code_of(out_dtype))
+    return out
+
+
+def _pass_gradient(grad: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
+    g = _dense(grad.detach())
+    out = torch.empty_like(g)
+    _lib.call("lq_mx_fake_quantize_grad", g.device, g.data_ptr(), _lib.code_of(g.dtype), mask.data_ptr(), g.numel(),
+              out.data_ptr())
     return out
 
 
@@ -97,11 +111,7 @@ class _StraightThrough(torch.autograd.Function):
     @staticmethod
     def forward(ctx, grad, mask):
         ctx.save_for_backward(mask)
-        g = _dense(grad.detach())
-        out = torch.empty_like(g)
-        _lib.call("lq_mx_fake_quantize_grad", g.device, g.data_ptr(), _lib.code_of(g.dtype), mask.data_ptr(), g.numel(),
-              out.data_ptr())
-        return out
+        return _pass_gradient(grad, mask)
 
     @staticmethod
     def backward(ctx, grad):
@@ -127,7 +137,9 @@ class _MXFakeQuantize(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         (mask,) = ctx.saved_tensors
-        return _StraightThrough.apply(grad, mask)
+        if torch.is_grad_enabled():  # create_graph: somebody differentiates the gradient
+            return _StraightThrough.apply(grad, mask)
+        return _pass_gradient(grad, mask)
 
 
 def mx_fake_quantize(x: torch.Tensor) -> torch.Tensor:
@@ -145,8 +157,10 @@ def _bias_of(bias, n: int, device) -> torch.Tensor | None:
     _lib.require_cuda(bias, "bias")
     if bias.device != device:
         raise _lib.DeviceMismatch(f"bias on {bias.device}, the product runs on {device}")
-    if tuple(bias.shape) != (n,):
+    if bias.dim() != 1 or bias.shape[0] != n:
         raise _lib.ShapeMismatch(f"bias is {tuple(bias.shape)}, expected {(n,)}")
+    if bias.dtype == torch.float32 and bias.is_contiguous():
+        return bias
     return bias.detach().to(torch.float32).contiguous()
 
 
@@ -162,12 +176,13 @@ def mx_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tens
         raise _lib.ShapeMismatch(f"the weight's codes must be (N, K / 2), got {tuple(w_codes.shape)}")
     if k != kw:
         raise _lib.ShapeMismatch(f"the left operand has {k} features, the weight {kw}")
-    if w_codes.device != a_codes.device:
-        raise _lib.DeviceMismatch(f"left operand on {a_codes.device}, weight on {w_codes.device}")
-    b = _bias_of(bias, n, a_codes.device)
-    out = torch.empty((*a_codes.shape[:-1], n), dtype=out_dtype, device=a_codes.device)
-    _lib.call("lq_mx_matmul", a_codes.device, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
-          int(relu), out.data_ptr(), _lib.code_of(out_dtype), n, _lib.status_word(a_codes.device).data_ptr())
+    dev = a_codes.device
+    if w_codes.device != dev:
+        raise _lib.DeviceMismatch(f"left operand on {dev}, weight on {w_codes.device}")
+    b = _bias_of(bias, n, dev)
+    out = torch.empty(*a_codes.shape[:-1], n, dtype=out_dtype, device=dev)
+    _lib.call("lq_mx_matmul", dev, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
+              int(relu), out.data_ptr(), _lib.code_of(out_dtype), n, _lib.status_word(dev).data_ptr())
     return out
 
 
@@ -180,15 +195,15 @@ def mx_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bi
         raise _lib.ShapeMismatch(f"the weight's codes must be (N, K / 2), got {tuple(w_codes.shape)}")
     if x.shape[-1] != k:
         raise _lib.ShapeMismatch(f"the input has {x.shape[-1]} features, the weight {k}")
-    if w_codes.device != x.device:
-        raise _lib.DeviceMismatch(f"input on {x.device}, weight on {w_codes.device}")
-    b = _bias_of(bias, n, x.device)
-    x2 = _rows(x)
-    m = x2.shape[0]
-    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    dev = x.device
+    if w_codes.device != dev:
+        raise _lib.DeviceMismatch(f"input on {dev}, weight on {w_codes.device}")
+    b = _bias_of(bias, n, dev)
+    x2, m, _, ld = _rows(x)
+    out = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
     room = (m * (k // 2) + 1023) // 1024 * 1024 + (m + 127) // 128 * ((k + 255) // 256) * 1024
-    ws = torch.empty(room, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(room, dtype=torch.uint8, device=dev)
     code = _lib.code_of(x.dtype)
-    _lib.call("lq_mx_linear", x.device, x2.data_ptr(), code, m, x2.stride(0), wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
-          int(relu), out.data_ptr(), code, n, ws.data_ptr(), room, _lib.status_word(x.device).data_ptr())
+    _lib.call("lq_mx_linear", dev, x2.data_ptr(), code, m, ld, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
+              int(relu), out.data_ptr(), code, n, ws.data_ptr(), room, _lib.status_word(dev).data_ptr())
     return out

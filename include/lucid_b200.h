@@ -481,7 +481,7 @@ int lq_mx_quantize(const void* x, int in_dtype, size_t rows, size_t K, size_t ld
 int lq_mx_dequantize(const uint8_t* codes, const uint8_t* scales, size_t rows, size_t K, void* out,
                      int out_dtype, void* stream);
 /* out = decode(encode(x)) over n contiguous values (n a multiple of 32), out of x's dtype.  mask
- * (optional, n / 8 bytes): bit i of byte j is set where value 8j + i was rounded inside the grid
+ * (optional, n / 8 bytes, 2-byte aligned): bit i of byte j is set where value 8j + i was rounded inside the grid
  * (|x| / scale < 7), the values whose gradient passes straight through. */
 int lq_mx_fake_quantize(const void* x, int dtype, size_t n, void* out, uint8_t* mask, void* stream);
 /* out = grad where the mask bit is set, 0 elsewhere. */

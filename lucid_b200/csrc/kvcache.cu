@@ -15,6 +15,7 @@ using mx::Chunk;
 using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256;
+constexpr int kWriteThreads = 512;
 constexpr int kMaxDim = 1024;
 
 struct Side {          // keys or values
@@ -30,6 +31,14 @@ __device__ __forceinline__ long long index_at(const void* p, int bits, size_t i)
   return bits == 64 ? __ldg(reinterpret_cast<const long long*>(p) + i) : (long long)__ldg(reinterpret_cast<const int*>(p) + i);
 }
 
+// n / d for n * d < 2^40, by a multiplication
+struct FastDiv {
+  uint32_t d;
+  unsigned long long m;  // ceil(2^40 / d)
+  __host__ explicit FastDiv(uint32_t div) : d(div), m((((unsigned long long)1 << 40) + div - 1) / div) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 40); }
+};
+
 // ---- write ---------------------------------------------------------------------------------------------
 
 // When a slot occurs more than once in a call, the last of its tokens is the one that is kept: each CTA
@@ -38,7 +47,7 @@ __device__ __forceinline__ long long index_at(const void* p, int bits, size_t i)
 // does not depend on their timing.
 template <int TOKENS>
 struct SlotTable {
-  static constexpr int kSize = 2 * TOKENS;
+  static constexpr int kSize = 4 * TOKENS;
   long long slot[TOKENS];   // slots of the CTA's tokens; -1: nothing is written
   int head[kSize];          // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
   int dead[TOKENS];         // a later token writes the same slot
@@ -50,75 +59,115 @@ __device__ __forceinline__ uint32_t slot_hash(long long s) {
   return h ^ (h >> 15);
 }
 
-template <typename T, bool MXF>
-__device__ __forceinline__ void encode_row(const Side& sd, long long token, long long slot, int head, int heads, int dim,
-                                           int group, int sub, uint32_t lanes) {
-  // `group` lanes (a power of two) hold a row of one head, eight values at a time
-  const T* x = reinterpret_cast<const T*>(sd.x) + token * sd.x_token + head * sd.x_head;
-  const int chunks = dim / 8;
-  const size_t row = (size_t)slot * heads + head;
-  if (MXF) {
-    for (int c0 = 0; c0 < chunks; c0 += group) {  // every lane of the group takes every step (shuffles)
-      const int c = c0 + sub;
-      Chunk<T> v;
-      const bool ok = c < chunks;
-      if (ok) v.load(x + c * 8);
-      else v.clear();
-      uint32_t amax = v.amax_bits();
-      amax = max(amax, __shfl_xor_sync(lanes, amax, 1));
-      amax = max(amax, __shfl_xor_sync(lanes, amax, 2));
-      const uint32_t byte = mx::scale_byte(amax);
-      float f[8];
-      v.values(f);
-      const float inv = mx::inverse_scale(byte);
+// A row of one head as its group of `group` lanes (a power of two) holds it: lane `sub` has the chunks sub,
+// sub + group, .. of sixteen values.
+template <typename T, int CHUNKS>
+struct Row {
+  Chunk<T> c[CHUNKS];
+  __device__ __forceinline__ void load(const T* x, int chunks, int group, int sub, bool ok, int wide) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
-      if (ok) {
-        reinterpret_cast<uint32_t*>(sd.codes + row * (dim / 2))[c] = byte == 255u ? 0u : mx::encode8(f);
-        if ((c & 3) == 0) sd.scales[row * (dim / 32) + c / 4] = (uint8_t)byte;
+    for (int i = 0; i < CHUNKS; ++i) {
+      if (ok && sub + i * group < chunks) c[i].load(x + (sub + i * group) * 16, wide);
+      else c[i].clear();
+    }
+  }
+};
+
+// Encode a row and store it at `row` of the cache.  Every lane of the group takes part (shuffles); `ok` says
+// whether the row is written.
+template <typename T, bool MXF, int CHUNKS>
+__device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>& x, size_t row, int dim, int group, int sub,
+                                           uint32_t lanes, bool ok) {
+  const int chunks = dim / 16;
+  if (MXF) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = sub + i * group;
+      const uint32_t byte = mx::block_byte<T>(x.c[i], lanes);
+      if (ok && c < chunks) {
+        reinterpret_cast<uint2*>(sd.codes + row * (dim / 2))[c] = mx::encode16<T>(x.c[i], byte);
+        if ((c & 1) == 0) sd.scales[row * (dim / 32) + c / 2] = (uint8_t)byte;
       }
     }
   } else {
-    uint32_t amax = 0;
-    for (int c = sub; c < chunks; c += group) {
-      Chunk<T> v;
-      v.load(x + c * 8);
-      amax = max(amax, v.amax_bits());
-    }
-    for (int o = group >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(lanes, amax, o));
+    uint32_t m = x.c[0].amax();
+#pragma unroll
+    for (int i = 1; i < CHUNKS; ++i) m = Chunk<T>::merge(m, x.c[i].amax());
+    for (int o = group >> 1; o > 0; o >>= 1) m = Chunk<T>::merge(m, __shfl_xor_sync(lanes, m, o));
+    if (!ok) return;
+    const uint32_t amax = Chunk<T>::amax_bits(m);
     // the arithmetic of the per-token encode on the grid [-128, 127]; a row that holds a NaN or an
     // infinity has no scale and reads back as NaN
     const float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu)
                                             : fmaxf(__fdiv_rn(__uint_as_float(amax), 127.5f), 1e-8f);
     const Divisor d = make_divisor(scale);
-    for (int c = sub; c < chunks; c += group) {
-      Chunk<T> v;
-      v.load(x + c * 8);
-      float f[8];
-      v.values(f);
-      uint32_t w[2];
+    const IntGrid grid = make_int_grid(0.0f, -128.0f, 127.0f, -128, 127);
+    const ShortDiv by_scale = make_short_div(d);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = sub + i * group;
+      if (c >= chunks) continue;
+      uint32_t w[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float x4[4] = {f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]};
-        float q[4];
-        code4_f32(x4, d, 0.0f, -128.0f, 127.0f, q);
-        w[h] = pack4_s8(q);
+        float f[8];
+        x.c[i].values(h, f);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x4[4] = {f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]};
+          if (d.fast) {  // every quotient is at most 127.5 in magnitude
+            int q[4];
+            code4_short(x4, by_scale, grid, q);
+            w[2 * h + j] = pack4i_s8(q);
+          } else {
+            float q[4];
+            code4_f32(x4, d, 0.0f, -128.0f, 127.0f, q);
+            w[2 * h + j] = pack4_s8(q);
+          }
+        }
       }
-      reinterpret_cast<uint2*>(sd.codes + row * dim)[c] = make_uint2(w[0], w[1]);
+      reinterpret_cast<uint4*>(sd.codes + row * dim)[c] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (sub == 0) reinterpret_cast<float*>(sd.scales)[row] = scale;
   }
 }
 
-template <typename T, bool MXF, int TOKENS>
-__global__ void __launch_bounds__(kThreads)
+// A CTA takes TOKENS tokens (and with gridDim.y > 1 a share of the heads).  The loads of its first rows are on
+// their way while the table of slots is built; a group of lanes keeps four rows of bf16 (128 bytes a lane) in
+// flight.
+template <typename T, bool MXF, int TOKENS, int CHUNKS>
+__global__ void __launch_bounds__(kWriteThreads)
 kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, size_t tokens, long long n_slots,
-                int heads, int dim, int group, int32_t* status) {
+                int heads, int dim, int group, const FastDiv per_token, int wide, int32_t* status) {
+  constexpr int kInFlight = 8 / (int)sizeof(T) / CHUNKS;
   __shared__ SlotTable<TOKENS> tab;
   const size_t t0 = (size_t)blockIdx.x * TOKENS;
   const int mine = (int)(tokens - t0 < (size_t)TOKENS ? tokens - t0 : (size_t)TOKENS);
-  for (int i = threadIdx.x; i < SlotTable<TOKENS>::kSize; i += kThreads) tab.head[i] = 0;
-  for (int i = threadIdx.x; i < mine; i += kThreads) {
+  const int per = (int)per_token.d / 2, h0 = blockIdx.y * per, here = min(per, heads - h0);  // heads of this CTA
+  const int lane = threadIdx.x & 31, sub = lane & (group - 1);
+  const uint32_t lanes = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (lane & ~(group - 1));
+  const int groups = kWriteThreads / group, rows = mine * (int)per_token.d;  // (token, head, side)
+  const int r_first = (int)threadIdx.x / group;
+  Row<T, CHUNKS> x[kInFlight];
+  auto place = [&](int r, int& token, int& head, int& side) {
+    token = (int)per_token((uint32_t)r);
+    const int w = r - token * (int)per_token.d;
+    side = w & 1, head = w >> 1;
+    return r < rows && head < here;
+  };
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      int token, head, side;
+      const bool ok = place(r0 + u * groups, token, head, side);
+      const Side& sd = side ? v : k;
+      x[u].load(reinterpret_cast<const T*>(sd.x) + (long long)(t0 + token) * sd.x_token + (h0 + head) * sd.x_head, dim / 16, group, sub, ok, wide);
+    }
+  };
+  load(r_first);
+
+  for (int i = threadIdx.x; i < SlotTable<TOKENS>::kSize; i += kWriteThreads) tab.head[i] = 0;
+  for (int i = threadIdx.x; i < mine; i += kWriteThreads) {
     long long s = index_at(slots, slot_bits, t0 + i);
     if (s >= n_slots) {
       s = -1;
@@ -128,7 +177,7 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
     tab.dead[i] = 0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < mine; i += kThreads) {
+  for (int i = threadIdx.x; i < mine; i += kWriteThreads) {
     const long long s = tab.slot[i];
     if (s < 0) continue;
     for (uint32_t h = slot_hash(s) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
@@ -142,42 +191,40 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
     }
   }
   __syncthreads();
-  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kThreads) {
-    const long long s = index_at(slots, slot_bits, t);
-    if (s < 0) continue;
-    for (uint32_t h = slot_hash(s) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
-      const int e = tab.head[h];
-      if (e == 0) break;
-      if (tab.slot[e - 1] == s) {
-        tab.dead[e - 1] = 1;
-        break;
+  constexpr int kAhead = 4;
+  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kAhead * kWriteThreads) {
+    long long s[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) s[j] = t + j * kWriteThreads < tokens ? index_at(slots, slot_bits, t + j * kWriteThreads) : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (s[j] < 0) continue;
+      for (uint32_t h = slot_hash(s[j]) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
+        const int e = tab.head[h];
+        if (e == 0) break;
+        if (tab.slot[e - 1] == s[j]) {
+          tab.dead[e - 1] = 1;
+          break;
+        }
       }
     }
   }
   __syncthreads();
-  // rows of this CTA: (token, head) of its share of the heads, keys then values
-  const int hs = (heads + gridDim.y - 1) / gridDim.y, h0 = blockIdx.y * hs, h1 = min(heads, h0 + hs);
-  if (h0 >= h1) return;
-  const int per = h1 - h0, lane = threadIdx.x & 31;
-  const int sub = lane & (group - 1);
-  const uint32_t lanes = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (lane & ~(group - 1));
-  const int rows = mine * per * 2;
-  for (int r = (int)threadIdx.x / group; r < rows; r += kThreads / group) {
-    const int side = r & 1, i = (r >> 1) / per, head = h0 + (r >> 1) % per;
-    if (tab.slot[i] < 0 || tab.dead[i]) continue;
-    encode_row<T, MXF>(side ? v : k, (long long)(t0 + i), tab.slot[i], head, heads, dim, group, sub, lanes);
+
+  for (int r0 = r_first; r0 - r_first < rows; r0 += kInFlight * groups) {
+    if (r0 != r_first) load(r0);
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      int token, head, side;
+      bool ok = place(r0 + u * groups, token, head, side);
+      const long long s = ok ? tab.slot[token] : -1;
+      ok = ok && s >= 0 && !tab.dead[token];
+      encode_row<T, MXF, CHUNKS>(side ? v : k, x[u], (size_t)(ok ? s : 0) * heads + h0 + head, dim, group, sub, lanes, ok);
+    }
   }
 }
 
 // ---- read ----------------------------------------------------------------------------------------------
-
-// n / d for n * d < 2^40, by a multiplication
-struct FastDiv {
-  uint32_t d;
-  unsigned long long m;  // ceil(2^40 / d)
-  __host__ explicit FastDiv(uint32_t div) : d(div), m((((unsigned long long)1 << 40) + div - 1) / div) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 40); }
-};
 
 struct Table {
   const int* pages;
@@ -291,24 +338,33 @@ int check_format(const std::string& w, int format, size_t heads, size_t dim) {
   return LQ_OK;
 }
 
-template <typename T, bool MXF, int TOKENS>
+template <typename T, bool MXF, int TOKENS, int CHUNKS>
 int write_tokens(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
-                 int dim, int group, int32_t* status, cudaStream_t st) {
+                 int dim, int group, int wide, int32_t* status, cudaStream_t st) {
   const size_t tiles = (tokens + TOKENS - 1) / TOKENS;
   if (tiles > 0x7fffffffu) return fail(LQ_ERR_SHAPE, "lq_kv_write: too many tokens for one launch");
-  unsigned split = 1;
-  while (tiles * split < 2 * (size_t)kNumSMs && split < (unsigned)heads) split *= 2;
-  kv_write_kernel<T, MXF, TOKENS><<<dim3((unsigned)tiles, split), kThreads, 0, st>>>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status);
+  // heads shared out until every SM has a CTA: a share repeats the table, but reads other rows
+  int per = heads;
+  while (per > 1 && tiles * (size_t)((heads + per - 1) / per) < (size_t)sm_count()) per = (per + 1) / 2;
+  kv_write_kernel<T, MXF, TOKENS, CHUNKS><<<dim3((unsigned)tiles, (unsigned)((heads + per - 1) / per)), kWriteThreads, 0, st>>>(
+      k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, FastDiv(2 * (uint32_t)per), wide, status);
   return check_cuda(cudaGetLastError(), "lq_kv_write launch");
+}
+template <typename T, bool MXF, int CHUNKS>
+int write_chunks(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
+                 int dim, int group, int wide, int32_t* status, cudaStream_t st) {
+  // Every CTA looks at the slots of all later tokens, so its share of the tokens grows with their number.
+  if (tokens <= 4096) return write_tokens<T, MXF, 16, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  if (tokens <= 32768) return write_tokens<T, MXF, 64, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  return write_tokens<T, MXF, 512, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
 }
 template <typename T, bool MXF>
 int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
-                   int dim, int32_t* status, cudaStream_t st) {
-  int group = 1;
-  while (group < 32 && group * 8 < dim) group *= 2;
-  if (tokens <= 4096) return write_tokens<T, MXF, 16>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
-  if (tokens <= 32768) return write_tokens<T, MXF, 128>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
-  return write_tokens<T, MXF, 1024>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, status, st);
+                   int dim, int wide, int32_t* status, cudaStream_t st) {
+  int group = MXF ? 2 : 1;
+  while (group < 32 && group * 16 < dim) group *= 2;
+  if (dim <= 512) return write_chunks<T, MXF, 1>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  return write_chunks<T, MXF, 2>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
 }
 
 }  // namespace
@@ -333,11 +389,13 @@ extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t to
   Side vs = {v, (long long)v_token, (long long)v_head, (uint8_t*)v_codes, (uint8_t*)v_scales, nullptr, 0, 0};
   cudaStream_t st = (cudaStream_t)stream;
   const int h = (int)heads, d = (int)dim;
+  const int wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 32 == 0) &&
+                   ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
   if (in_dtype == LQ_F32)
-    return format == LQ_KV_MXFP4 ? write_dispatch<float, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st)
-                                 : write_dispatch<float, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st);
-  return format == LQ_KV_MXFP4 ? write_dispatch<bf16, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st)
-                               : write_dispatch<bf16, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, status, st);
+    return format == LQ_KV_MXFP4 ? write_dispatch<float, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st)
+                                 : write_dispatch<float, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st);
+  return format == LQ_KV_MXFP4 ? write_dispatch<bf16, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st)
+                               : write_dispatch<bf16, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st);
 }
 
 extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int format,

@@ -70,64 +70,106 @@ __device__ __forceinline__ void decode8(uint32_t codes, float (&v)[8]) {
   }
 }
 
-// The element nearest to a scaled value (magnitude below 8), as a value.  The grid's spacing is 1/2 below
-// 2, 1 below 4 and 2 above; adding and subtracting 1.5 * 2^23 spacings rounds to a multiple of it, ties to
-// the even multiple, which is the even mantissa.  (encode8 followed by decode8 in one kernel came out as
-// zeros from this toolchain; through memory the pair is right.)
-__device__ __forceinline__ float round_element(float t) {
-  const float a = fabsf(t);
-  const float m = a < 2.0f ? 6291456.0f : (a < 4.0f ? 12582912.0f : 25165824.0f);
-  return copysignf(fminf(__fsub_rn(__fadd_rn(a, m), m), 6.0f), t);
-}
-
-// Eight consecutive values of a thread, kept as they were loaded.
+// Sixteen consecutive values of a thread, kept as they were loaded; two threads hold a block.  `amax` is the
+// largest magnitude in a form that `merge` combines and `amax_bits` turns into a float32 bit pattern ordered
+// like the magnitudes, a NaN above infinity.
 template <typename T>
 struct Chunk;
 template <>
 struct Chunk<float> {
-  uint4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  uint32_t w[16];
+  __device__ __forceinline__ void load(const float* p, int wide) {
+    if (wide) {  // 32-byte aligned
+#pragma unroll
+      for (int i = 0; i < 16; i += 8)
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                     : "l"(p + i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const uint4 v = ld_stream_u4(p + i);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    }
   }
-  // one 32-byte load: p is 32-byte aligned
-  __device__ __forceinline__ void load_wide(const float* p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
-                 : "l"(p));
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 0;
   }
-  __device__ __forceinline__ void clear() { a = b = make_uint4(0, 0, 0, 0); }
-  // float32 bit pattern of the largest magnitude (ordered like the magnitudes, NaN above infinity)
-  __device__ __forceinline__ uint32_t amax_bits() const {
-    const uint32_t m = 0x7fffffffu;
-    return max(max(max(a.x & m, a.y & m), max(a.z & m, a.w & m)), max(max(b.x & m, b.y & m), max(b.z & m, b.w & m)));
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = w[0] & 0x7fffffffu;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
   }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+  static __device__ __forceinline__ uint32_t merge(uint32_t a, uint32_t b) { return max(a, b); }
+  static __device__ __forceinline__ uint32_t amax_bits(uint32_t m) { return m; }
+  __device__ __forceinline__ void values(int half, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[8 * half + i]);
   }
 };
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 template <>
 struct Chunk<__nv_bfloat16> {
-  uint4 a;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = ld_stream_u4(p); }
-  __device__ __forceinline__ void load_wide(const __nv_bfloat16* p) { load(p); }
-  __device__ __forceinline__ void clear() { a = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ uint32_t amax_bits() const {
-    const uint32_t m = 0x7fff7fffu;
-    const uint32_t t = max_u16x2(max_u16x2(a.x & m, a.y & m), max_u16x2(a.z & m, a.w & m));
-    return max(t << 16, t & 0xffff0000u);
-  }
-  __device__ __forceinline__ void values(float (&v)[8]) const {
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  uint32_t w[8];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int wide) {
+    if (wide) {
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 8; i += 4) {
+        const uint4 v = ld_stream_u4(p + 2 * i);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+  }
+  // pairwise: two halves a word until the very end
+  static __device__ __forceinline__ uint32_t merge(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = merge(m, w[i] & 0x7fff7fffu);
+    return m;
+  }
+  static __device__ __forceinline__ uint32_t amax_bits(uint32_t m) { return max(m << 16, m & 0xffff0000u); }
+  __device__ __forceinline__ void values(int half, float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[2 * i] = __uint_as_float(w[4 * half + i] << 16), v[2 * i + 1] = __uint_as_float(w[4 * half + i] & 0xffff0000u);
   }
 };
+// The block's scale byte, known to both threads that hold it (`lanes`: the threads that call this together).
+template <typename T>
+__device__ __forceinline__ uint32_t block_byte(const Chunk<T>& c, uint32_t lanes) {
+  const uint32_t m = c.amax();
+  return scale_byte(Chunk<T>::amax_bits(Chunk<T>::merge(m, __shfl_xor_sync(lanes, m, 1))));
+}
+// Codes of the sixteen values, value i in bits [4i, 4i + 4); zero for a block without a scale.
+template <typename T>
+__device__ __forceinline__ uint2 encode16(const Chunk<T>& c, uint32_t byte) {
+  const float inv = inverse_scale(byte);
+  uint32_t q[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+    c.values(h, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], inv);
+    q[h] = encode8(v);
+  }
+  return byte == 255u ? make_uint2(0, 0) : make_uint2(q[0], q[1]);
+}
 
 // Eight values -> memory (16-byte aligned), rounded once when T is narrower.
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
@@ -159,7 +201,6 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8], int wide) 
     store8(p, v);
   }
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8], int) { store8(p, v); }
 // Sixteen values.
 __device__ __forceinline__ void store16(float* p, const float (&lo)[8], const float (&hi)[8], int wide) {
   store8(p, lo, wide);

@@ -15,18 +15,14 @@ using mx::Chunk;
 using bf16 = __nv_bfloat16;
 
 constexpr int kThreads = 256;
-constexpr int kWriteThreads = 512;
 constexpr int kMaxDim = 1024;
 
-struct Side {          // keys or values
-  const void* x;       // new rows (write) / unused
-  long long x_token, x_head;
+struct Side {           // keys or values
   uint8_t* codes;
-  uint8_t* scales;     // float32 (int8 format) or scale bytes
-  void* out;           // read: destination
-  long long out_token, out_head;
+  uint8_t* scales;      // float32 (int8 format) or scale bytes
+  void* rows;           // new rows (write), output rows (read)
+  long long token, head;  // their strides
 };
-
 __device__ __forceinline__ long long index_at(const void* p, int bits, size_t i) {
   return bits == 64 ? __ldg(reinterpret_cast<const long long*>(p) + i) : (long long)__ldg(reinterpret_cast<const int*>(p) + i);
 }
@@ -44,13 +40,14 @@ struct FastDiv {
 // When a slot occurs more than once in a call, the last of its tokens is the one that is kept: each CTA
 // enters its tokens' slots into a hash table in shared memory (the latest token of a slot wins there) and
 // looks the slots of all later tokens up in it.  The rule needs no state between launches and its result
-// does not depend on their timing.
+// does not depend on their timing.  The table is thirty-two times too large, so that a slot which is not in it
+// is nearly always told by one look.
 template <int TOKENS>
 struct SlotTable {
-  static constexpr int kSize = 4 * TOKENS;
-  long long slot[TOKENS];   // slots of the CTA's tokens; -1: nothing is written
-  int head[kSize];          // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
-  int dead[TOKENS];         // a later token writes the same slot
+  static constexpr uint32_t kSize = 32 * TOKENS;
+  long long slot[TOKENS];       // slots of the CTA's tokens; -1: nothing is written
+  unsigned short head[kSize];   // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
+  uint8_t dead[TOKENS];         // a later token writes the same slot
 };
 
 __device__ __forceinline__ uint32_t slot_hash(long long s) {
@@ -73,17 +70,18 @@ struct Row {
   }
 };
 
-// Encode a row and store it at `row` of the cache.  Every lane of the group takes part (shuffles); `ok` says
-// whether the row is written.
+// Encode a row and store it at `row` of the cache.  Every lane of the warp takes part (shuffles, whose mask is
+// the constant full one: a mask that names the group costs a synchronisation unit's round trip each);
+// `ok` says whether the row is written.
 template <typename T, bool MXF, int CHUNKS>
 __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>& x, size_t row, int dim, int group, int sub,
-                                           uint32_t lanes, bool ok) {
+                                           bool ok) {
   const int chunks = dim / 16;
   if (MXF) {
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int c = sub + i * group;
-      const uint32_t byte = mx::block_byte<T>(x.c[i], lanes);
+      const uint32_t byte = mx::block_byte<T>(x.c[i]);
       if (ok && c < chunks) {
         reinterpret_cast<uint2*>(sd.codes + row * (dim / 2))[c] = mx::encode16<T>(x.c[i], byte);
         if ((c & 1) == 0) sd.scales[row * (dim / 32) + c / 2] = (uint8_t)byte;
@@ -93,7 +91,7 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
     uint32_t m = x.c[0].amax();
 #pragma unroll
     for (int i = 1; i < CHUNKS; ++i) m = Chunk<T>::merge(m, x.c[i].amax());
-    for (int o = group >> 1; o > 0; o >>= 1) m = Chunk<T>::merge(m, __shfl_xor_sync(lanes, m, o));
+    for (int o = group >> 1; o > 0; o >>= 1) m = Chunk<T>::merge(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (!ok) return;
     const uint32_t amax = Chunk<T>::amax_bits(m);
     // the arithmetic of the per-token encode on the grid [-128, 127]; a row that holds a NaN or an
@@ -112,18 +110,19 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
       for (int h = 0; h < 2; ++h) {
         float f[8];
         x.c[i].values(h, f);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float x4[4] = {f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]};
-          if (d.fast) {  // every quotient is at most 127.5 in magnitude
-            int q[4];
-            code4_short(x4, by_scale, grid, q);
-            w[2 * h + j] = pack4i_s8(q);
-          } else {
-            float q[4];
-            code4_f32(x4, d, 0.0f, -128.0f, 127.0f, q);
-            w[2 * h + j] = pack4_s8(q);
-          }
+        const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
+        if (d.fast) {  // every quotient is at most 127.5 in magnitude
+          int q[4];
+          code4_short(a, by_scale, grid, q);
+          w[2 * h] = pack4i_s8(q);
+          code4_short(b, by_scale, grid, q);
+          w[2 * h + 1] = pack4i_s8(q);
+        } else {
+          float q[4];
+          code4_f32(a, d, 0.0f, -128.0f, 127.0f, q);
+          w[2 * h] = pack4_s8(q);
+          code4_f32(b, d, 0.0f, -128.0f, 127.0f, q);
+          w[2 * h + 1] = pack4_s8(q);
         }
       }
       reinterpret_cast<uint4*>(sd.codes + row * dim)[c] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -136,7 +135,7 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 // their way while the table of slots is built; a group of lanes keeps four rows of bf16 (128 bytes a lane) in
 // flight.
 template <typename T, bool MXF, int TOKENS, int CHUNKS>
-__global__ void __launch_bounds__(kWriteThreads)
+__global__ void __launch_bounds__(kThreads)
 kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, size_t tokens, long long n_slots,
                 int heads, int dim, int group, const FastDiv per_token, int wide, int32_t* status) {
   constexpr int kInFlight = 8 / (int)sizeof(T) / CHUNKS;
@@ -145,8 +144,7 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
   const int mine = (int)(tokens - t0 < (size_t)TOKENS ? tokens - t0 : (size_t)TOKENS);
   const int per = (int)per_token.d / 2, h0 = blockIdx.y * per, here = min(per, heads - h0);  // heads of this CTA
   const int lane = threadIdx.x & 31, sub = lane & (group - 1);
-  const uint32_t lanes = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (lane & ~(group - 1));
-  const int groups = kWriteThreads / group, rows = mine * (int)per_token.d;  // (token, head, side)
+  const int groups = kThreads / group, rows = mine * (int)per_token.d;  // (token, head, side)
   const int r_first = (int)threadIdx.x / group;
   Row<T, CHUNKS> x[kInFlight];
   auto place = [&](int r, int& token, int& head, int& side) {
@@ -161,13 +159,14 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
       int token, head, side;
       const bool ok = place(r0 + u * groups, token, head, side);
       const Side& sd = side ? v : k;
-      x[u].load(reinterpret_cast<const T*>(sd.x) + (long long)(t0 + token) * sd.x_token + (h0 + head) * sd.x_head, dim / 16, group, sub, ok, wide);
+      x[u].load(reinterpret_cast<const T*>(sd.rows) + (long long)(t0 + token) * sd.token + (h0 + head) * sd.head, dim / 16, group, sub, ok, wide);
     }
   };
   load(r_first);
 
-  for (int i = threadIdx.x; i < SlotTable<TOKENS>::kSize; i += kWriteThreads) tab.head[i] = 0;
-  for (int i = threadIdx.x; i < mine; i += kWriteThreads) {
+  constexpr uint32_t kSize = SlotTable<TOKENS>::kSize;
+  for (uint32_t i = threadIdx.x; i < kSize / 8; i += kThreads) reinterpret_cast<uint4*>(tab.head)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < mine; i += kThreads) {
     long long s = index_at(slots, slot_bits, t0 + i);
     if (s >= n_slots) {
       s = -1;
@@ -177,29 +176,33 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
     tab.dead[i] = 0;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < mine; i += kWriteThreads) {
+  for (int i = threadIdx.x; i < mine; i += kThreads) {
     const long long s = tab.slot[i];
     if (s < 0) continue;
-    for (uint32_t h = slot_hash(s) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
-      const int old = atomicCAS(&tab.head[h], 0, i + 1);
+    for (uint32_t h = slot_hash(s) % kSize;; h = (h + 1) % kSize) {
+      unsigned short old = atomicCAS(&tab.head[h], (unsigned short)0, (unsigned short)(i + 1));
       if (old == 0) break;
-      if (tab.slot[old - 1] == s) {  // the entry stays with this slot: keep its latest token
-        const int was = atomicMax(&tab.head[h], i + 1);
-        tab.dead[was < i + 1 ? was - 1 : i] = 1;
-        break;
+      if (tab.slot[old - 1] != s) continue;
+      // the entry stays with this slot: keep its latest token
+      while (old < i + 1) {
+        const unsigned short now = atomicCAS(&tab.head[h], old, (unsigned short)(i + 1));
+        if (now == old) break;
+        old = now;
       }
+      tab.dead[old < i + 1 ? old - 1 : i] = 1;
+      break;
     }
   }
   __syncthreads();
   constexpr int kAhead = 4;
-  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kAhead * kWriteThreads) {
+  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kAhead * kThreads) {
     long long s[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) s[j] = t + j * kWriteThreads < tokens ? index_at(slots, slot_bits, t + j * kWriteThreads) : -1;
+    for (int j = 0; j < kAhead; ++j) s[j] = t + j * kThreads < tokens ? index_at(slots, slot_bits, t + j * kThreads) : -1;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (s[j] < 0) continue;
-      for (uint32_t h = slot_hash(s[j]) % SlotTable<TOKENS>::kSize;; h = (h + 1) % SlotTable<TOKENS>::kSize) {
+      for (uint32_t h = slot_hash(s[j]) % kSize;; h = (h + 1) % kSize) {
         const int e = tab.head[h];
         if (e == 0) break;
         if (tab.slot[e - 1] == s[j]) {
@@ -219,7 +222,7 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
       bool ok = place(r0 + u * groups, token, head, side);
       const long long s = ok ? tab.slot[token] : -1;
       ok = ok && s >= 0 && !tab.dead[token];
-      encode_row<T, MXF, CHUNKS>(side ? v : k, x[u], (size_t)(ok ? s : 0) * heads + h0 + head, dim, group, sub, lanes, ok);
+      encode_row<T, MXF, CHUNKS>(side ? v : k, x[u], (size_t)(ok ? s : 0) * heads + h0 + head, dim, group, sub, ok);
     }
   }
 }
@@ -293,7 +296,7 @@ kv_read_kernel(const Side k, const Side v, const Table t, int heads, const FastD
       const uint32_t w = c - i * per_row.d, side = per_side(w), x = w - side * per_side.d;
       const uint32_t head = per_head(x), d0 = (x - head * per_head.d) * 16;
       const Side& sd = side ? v : k;
-      dst[u] = reinterpret_cast<T*>(sd.out) + (r0 + i) * sd.out_token + head * sd.out_head + d0;
+      dst[u] = reinterpret_cast<T*>(sd.rows) + (r0 + i) * sd.token + head * sd.head + d0;
       if (at[u] >= 0) {
         const size_t row = (size_t)at[u] * heads + head;
         if (MXF) {
@@ -345,8 +348,8 @@ int write_tokens(const Side& k, const Side& v, const void* slots, int slot_bits,
   if (tiles > 0x7fffffffu) return fail(LQ_ERR_SHAPE, "lq_kv_write: too many tokens for one launch");
   // heads shared out until every SM has a CTA: a share repeats the table, but reads other rows
   int per = heads;
-  while (per > 1 && tiles * (size_t)((heads + per - 1) / per) < (size_t)sm_count()) per = (per + 1) / 2;
-  kv_write_kernel<T, MXF, TOKENS, CHUNKS><<<dim3((unsigned)tiles, (unsigned)((heads + per - 1) / per)), kWriteThreads, 0, st>>>(
+  while (per > 1 && tiles * (size_t)((heads + per - 1) / per) < 2 * (size_t)sm_count()) per = (per + 1) / 2;
+  kv_write_kernel<T, MXF, TOKENS, CHUNKS><<<dim3((unsigned)tiles, (unsigned)((heads + per - 1) / per)), kThreads, 0, st>>>(
       k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, FastDiv(2 * (uint32_t)per), wide, status);
   return check_cuda(cudaGetLastError(), "lq_kv_write launch");
 }
@@ -354,9 +357,9 @@ template <typename T, bool MXF, int CHUNKS>
 int write_chunks(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
                  int dim, int group, int wide, int32_t* status, cudaStream_t st) {
   // Every CTA looks at the slots of all later tokens, so its share of the tokens grows with their number.
-  if (tokens <= 4096) return write_tokens<T, MXF, 16, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
-  if (tokens <= 32768) return write_tokens<T, MXF, 64, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
-  return write_tokens<T, MXF, 512, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  if (tokens <= 8192) return write_tokens<T, MXF, 16, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  if (tokens <= 65536) return write_tokens<T, MXF, 64, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+  return write_tokens<T, MXF, 256, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
 }
 template <typename T, bool MXF>
 int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
@@ -385,8 +388,8 @@ extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t to
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_write: rows of k and v must be 16-byte aligned");
   if (!aligned16(k_codes) || !aligned16(v_codes) || !aligned16(k_scales) || !aligned16(v_scales))
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_write: the cache must be 16-byte aligned");
-  Side ks = {k, (long long)k_token, (long long)k_head, (uint8_t*)k_codes, (uint8_t*)k_scales, nullptr, 0, 0};
-  Side vs = {v, (long long)v_token, (long long)v_head, (uint8_t*)v_codes, (uint8_t*)v_scales, nullptr, 0, 0};
+  const Side ks = {(uint8_t*)k_codes, (uint8_t*)k_scales, const_cast<void*>(k), (long long)k_token, (long long)k_head};
+  const Side vs = {(uint8_t*)v_codes, (uint8_t*)v_scales, const_cast<void*>(v), (long long)v_token, (long long)v_head};
   cudaStream_t st = (cudaStream_t)stream;
   const int h = (int)heads, d = (int)dim;
   const int wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 32 == 0) &&
@@ -416,8 +419,8 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_read: output rows must be 16-byte aligned");
   if (!aligned16(k_codes) || !aligned16(v_codes) || !aligned16(k_scales) || !aligned16(v_scales))
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_read: the cache must be 16-byte aligned");
-  Side ks = {nullptr, 0, 0, (uint8_t*)k_codes, (uint8_t*)k_scales, out_k, (long long)k_token, (long long)k_head};
-  Side vs = {nullptr, 0, 0, (uint8_t*)v_codes, (uint8_t*)v_scales, out_v, (long long)v_token, (long long)v_head};
+  const Side ks = {(uint8_t*)const_cast<void*>(k_codes), (uint8_t*)const_cast<void*>(k_scales), out_k, (long long)k_token, (long long)k_head};
+  const Side vs = {(uint8_t*)const_cast<void*>(v_codes), (uint8_t*)const_cast<void*>(v_scales), out_v, (long long)v_token, (long long)v_head};
   const Table t = {table, (long long)table_stride, (int)max_blocks, cu_seqlens, starts, (int)seqs, (long long)n_pages, (int)page};
   const uint32_t head_chunks = (uint32_t)(dim / 16), side_chunks = head_chunks * (uint32_t)heads;
   const int wide = ((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) % 32 == 0) &&

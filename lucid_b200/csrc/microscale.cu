@@ -51,7 +51,7 @@ mx_quantize_kernel(const T* __restrict__ x, size_t rows, size_t K, size_t ldx, u
   uint8_t* code_at = codes + row0 * (K / 2) + k0 / 2;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const uint32_t byte = mx::block_byte<T>(c[r], 0xffffffffu);
+    const uint32_t byte = mx::block_byte<T>(c[r]);
     const uint2 q = mx::encode16<T>(c[r], byte);
     if (in_k && row0 + r < rows) *reinterpret_cast<uint2*>(code_at + r * (K / 2)) = q;
     // lanes past K and rows past the end hold zeros and so byte 0
@@ -108,7 +108,7 @@ mx_fake_quantize_kernel(const T* __restrict__ x, size_t n, int wide, uint32_t ze
   Chunk<T> c;
   if (valid) c.load(x + i0, wide);
   else c.clear();
-  const uint32_t byte = mx::block_byte<T>(c, 0xffffffffu);
+  const uint32_t byte = mx::block_byte<T>(c);
   if (!valid) return;
   const float inv = mx::inverse_scale(byte), s = mx::scale_value(byte);
   float y[2][8];

@@ -149,11 +149,11 @@ struct Chunk<__nv_bfloat16> {
       v[2 * i] = __uint_as_float(w[4 * half + i] << 16), v[2 * i + 1] = __uint_as_float(w[4 * half + i] & 0xffff0000u);
   }
 };
-// The block's scale byte, known to both threads that hold it (`lanes`: the threads that call this together).
+// The block's scale byte, known to both threads that hold it.  The whole warp calls this.
 template <typename T>
-__device__ __forceinline__ uint32_t block_byte(const Chunk<T>& c, uint32_t lanes) {
+__device__ __forceinline__ uint32_t block_byte(const Chunk<T>& c) {
   const uint32_t m = c.amax();
-  return scale_byte(Chunk<T>::amax_bits(Chunk<T>::merge(m, __shfl_xor_sync(lanes, m, 1))));
+  return scale_byte(Chunk<T>::amax_bits(Chunk<T>::merge(m, __shfl_xor_sync(0xffffffffu, m, 1))));
 }
 // Codes of the sixteen values, value i in bits [4i, 4i + 4); zero for a block without a scale.
 template <typename T>

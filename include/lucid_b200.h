@@ -513,11 +513,13 @@ enum lq_kv_format { LQ_KV_INT8 = 0, LQ_KV_MXFP4 = 1 };
 /* Encode k and v, (tokens, heads, dim) with element strides (token, head) and contiguous dim, LQ_F32 |
  * LQ_BF16, into slots[0..tokens) (int32 or int64: slot_bits).  A negative slot is skipped (padding); a
  * slot >= n_slots is skipped and writes LQ_ERR_SHAPE to *status (optional).  A slot that occurs more
- * than once keeps the last of its tokens. */
+ * than once keeps the last of its tokens.  The workspace (any content; none for up to 256 tokens) marks the
+ * tokens that are overwritten. */
+size_t lq_kv_write_workspace_bytes(size_t tokens);
 int lq_kv_write(const void* k, const void* v, int in_dtype, size_t tokens, size_t heads, size_t dim, size_t k_token,
                 size_t k_head, size_t v_token, size_t v_head, const void* slots, int slot_bits, size_t n_slots,
-                int format, void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t* status,
-                void* stream);
+                int format, void* k_codes, void* k_scales, void* v_codes, void* v_scales, void* workspace,
+                size_t workspace_bytes, int32_t* status, void* stream);
 /* Decode `total` packed rows: row r with cu_seqlens[b] <= r < cu_seqlens[b + 1] (int32, seqs + 1 entries,
  * ascending) is position starts[b] (NULL: 0) + r - cu_seqlens[b] of sequence b, held in page
  * table[b * table_stride + position / page].  A position past the table's max_blocks columns or a page

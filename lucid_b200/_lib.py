@@ -154,7 +154,8 @@ _SIGNATURES = {
                                C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p,
                                C.c_size_t, C.c_void_p, C.c_void_p]),
     "lq_kv_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int] + [C.c_size_t] * 7 +
-                    [C.c_void_p, C.c_int, C.c_size_t, C.c_int] + [C.c_void_p] * 6),
+                    [C.c_void_p, C.c_int, C.c_size_t, C.c_int] + [C.c_void_p] * 5 + [C.c_size_t] + [C.c_void_p] * 2),
+    "lq_kv_write_workspace_bytes": (C.c_size_t, [C.c_size_t]),
     "lq_kv_read": (C.c_int, [C.c_void_p] * 4 + [C.c_int] + [C.c_size_t] * 4 + [C.c_void_p, C.c_size_t, C.c_size_t] +
                    [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int] +
                    [C.c_size_t] * 4 + [C.c_int, C.c_void_p, C.c_void_p]),

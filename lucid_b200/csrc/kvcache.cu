@@ -27,33 +27,90 @@ __device__ __forceinline__ long long index_at(const void* p, int bits, size_t i)
   return bits == 64 ? __ldg(reinterpret_cast<const long long*>(p) + i) : (long long)__ldg(reinterpret_cast<const int*>(p) + i);
 }
 
-// n / d for n * d < 2^40, by a multiplication
+// n / d for n * d < 2^43 (the rounding of m adds less than d * n / 2^43 < 1 / d to the quotient), n < 2^31, by the
+// upper half of a 64-bit product
 struct FastDiv {
   uint32_t d;
-  unsigned long long m;  // ceil(2^40 / d)
-  __host__ explicit FastDiv(uint32_t div) : d(div), m((((unsigned long long)1 << 40) + div - 1) / div) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((n * m) >> 40); }
+  unsigned long long m;  // 2^20 * ceil(2^43 / d)
+  __host__ explicit FastDiv(uint32_t div) : d(div), m(((((unsigned long long)1 << 43) + div - 1) / div) << 20) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)__umul64hi((unsigned long long)n << 1, m); }
 };
 
 // ---- write ---------------------------------------------------------------------------------------------
 
-// When a slot occurs more than once in a call, the last of its tokens is the one that is kept: each CTA
-// enters its tokens' slots into a hash table in shared memory (the latest token of a slot wins there) and
-// looks the slots of all later tokens up in it.  The rule needs no state between launches and its result
-// does not depend on their timing.  The table is thirty-two times too large, so that a slot which is not in it
-// is nearly always told by one look.
+// When a slot occurs more than once in a call, the last of its tokens is the one that is kept, whatever the
+// timing and without state between launches.  Up to kInline tokens, the warp that holds a token's rows compares
+// its slot with those of all later tokens itself; for more, a kernel of its own marks the tokens that are
+// overwritten: a CTA enters its tokens' slots into a hash table in shared memory (the latest token of a slot
+// wins there) and looks the slots of all later tokens up in it.  The table is many times too large, so that a
+// slot which is not in it is nearly always told by one look.  (Inside the write itself the looks and their
+// barriers cost 5 of 22 us at 8192 tokens, and more than the rows at 32.)
+constexpr int kInline = 256;
+constexpr int kMarkThreads = 1024;
 template <int TOKENS>
 struct SlotTable {
-  static constexpr uint32_t kSize = 32 * TOKENS;
-  long long slot[TOKENS];       // slots of the CTA's tokens; -1: nothing is written
-  unsigned short head[kSize];   // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
-  uint8_t dead[TOKENS];         // a later token writes the same slot
+  static constexpr uint32_t kSize = (TOKENS <= 256 ? 32 : 8) * TOKENS;
+  long long slot[TOKENS];                   // slots of the CTA's tokens; negative: nothing is written
+  alignas(16) unsigned short head[kSize];   // 0: empty, else 1 + local token whose slot this entry holds (the latest one)
+  uint8_t dead[TOKENS];                     // a later token writes the same slot
 };
 
 __device__ __forceinline__ uint32_t slot_hash(long long s) {
   uint32_t h = (uint32_t)s ^ (uint32_t)(s >> 32) * 0x9E3779B1u;
   h *= 0x85EBCA6Bu;
   return h ^ (h >> 15);
+}
+
+template <int TOKENS>
+__global__ void __launch_bounds__(kMarkThreads)
+kv_mark_kernel(const void* __restrict__ slots, int slot_bits, size_t tokens, uint8_t* __restrict__ dead) {
+  constexpr uint32_t kSize = SlotTable<TOKENS>::kSize;
+  __shared__ SlotTable<TOKENS> tab;
+  pdl_wait();
+  pdl_launch_dependents();
+  const size_t t0 = (size_t)blockIdx.x * TOKENS;
+  const int mine = (int)(tokens - t0 < (size_t)TOKENS ? tokens - t0 : (size_t)TOKENS);
+  for (uint32_t i = threadIdx.x; i < kSize / 8; i += kMarkThreads) reinterpret_cast<uint4*>(tab.head)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < mine; i += kMarkThreads) tab.slot[i] = index_at(slots, slot_bits, t0 + i), tab.dead[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine; i += kMarkThreads) {
+    const long long s = tab.slot[i];
+    if (s < 0) continue;
+    for (uint32_t h = slot_hash(s) % kSize;; h = (h + 1) % kSize) {
+      unsigned short old = atomicCAS(&tab.head[h], (unsigned short)0, (unsigned short)(i + 1));
+      if (old == 0) break;
+      if (tab.slot[old - 1] != s) continue;
+      // the entry stays with this slot: keep its latest token
+      while (old < i + 1) {
+        const unsigned short now = atomicCAS(&tab.head[h], old, (unsigned short)(i + 1));
+        if (now == old) break;
+        old = now;
+      }
+      tab.dead[old < i + 1 ? old - 1 : i] = 1;
+      break;
+    }
+  }
+  __syncthreads();
+  constexpr int kAhead = 4;
+  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kAhead * kMarkThreads) {
+    long long s[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) s[j] = t + j * kMarkThreads < tokens ? index_at(slots, slot_bits, t + j * kMarkThreads) : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (s[j] < 0) continue;
+      for (uint32_t h = slot_hash(s[j]) % kSize;; h = (h + 1) % kSize) {
+        const int e = tab.head[h];
+        if (e == 0) break;
+        if (tab.slot[e - 1] == s[j]) {
+          tab.dead[e - 1] = 1;
+          break;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine; i += kMarkThreads) dead[t0 + i] = tab.dead[i];
 }
 
 // A row of one head as its group of `group` lanes (a power of two) holds it: lane `sub` has the chunks sub,
@@ -74,8 +131,7 @@ struct Row {
 // the constant full one: a mask that names the group costs a synchronisation unit's round trip each);
 // `ok` says whether the row is written.
 template <typename T, bool MXF, int CHUNKS>
-__device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>& x, size_t row, int dim, int group, int sub,
-                                           bool ok) {
+__device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>& x, size_t row, int dim, int group, int sub, bool ok) {
   const int chunks = dim / 16;
   if (MXF) {
 #pragma unroll
@@ -94,13 +150,19 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
     for (int o = group >> 1; o > 0; o >>= 1) m = Chunk<T>::merge(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (!ok) return;
     const uint32_t amax = Chunk<T>::amax_bits(m);
-    // the arithmetic of the per-token encode on the grid [-128, 127]; a row that holds a NaN or an
-    // infinity has no scale and reads back as NaN
-    const float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu)
-                                            : fmaxf(__fdiv_rn(__uint_as_float(amax), 127.5f), 1e-8f);
-    const Divisor d = make_divisor(scale);
+    // The arithmetic of the per-token encode on the grid [-128, 127]: correctly rounded quotients by twice
+    // corrected reciprocals.  Every intermediate keeps its bits where a code depends on them: the scale is
+    // between 1e-8 and 2^121, a quotient at most 127.5, and an abs-max small enough to lose bits in the first
+    // division is below the 1e-8.  A row that holds a NaN or an infinity takes a NaN scale and reads back as NaN.
+    const float a = __uint_as_float(amax);
+    float q0 = __fmul_rn(a, 1.0f / 127.5f);
+    q0 = __fmaf_rn(__fmaf_rn(-q0, 127.5f, a), 1.0f / 127.5f, q0);
+    q0 = __fmaf_rn(__fmaf_rn(-q0, 127.5f, a), 1.0f / 127.5f, q0);
+    const float scale = amax >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fmaxf(q0, 1e-8f);
+    const float y = __frcp_rn(scale);
+    ShortDiv by_scale;
+    by_scale.y2 = f2_pack(y, y), by_scale.ns2 = f2_pack(-scale, -scale);
     const IntGrid grid = make_int_grid(0.0f, -128.0f, 127.0f, -128, 127);
-    const ShortDiv by_scale = make_short_div(d);
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       const int c = sub + i * group;
@@ -110,20 +172,12 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
       for (int h = 0; h < 2; ++h) {
         float f[8];
         x.c[i].values(h, f);
-        const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
-        if (d.fast) {  // every quotient is at most 127.5 in magnitude
-          int q[4];
-          code4_short(a, by_scale, grid, q);
-          w[2 * h] = pack4i_s8(q);
-          code4_short(b, by_scale, grid, q);
-          w[2 * h + 1] = pack4i_s8(q);
-        } else {
-          float q[4];
-          code4_f32(a, d, 0.0f, -128.0f, 127.0f, q);
-          w[2 * h] = pack4_s8(q);
-          code4_f32(b, d, 0.0f, -128.0f, 127.0f, q);
-          w[2 * h + 1] = pack4_s8(q);
-        }
+        const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+        int q[4];
+        code4_short(lo, by_scale, grid, q);
+        w[2 * h] = pack4i_s8(q);
+        code4_short(hi, by_scale, grid, q);
+        w[2 * h + 1] = pack4i_s8(q);
       }
       reinterpret_cast<uint4*>(sd.codes + row * dim)[c] = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -131,99 +185,65 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
   }
 }
 
-// A CTA takes TOKENS tokens (and with gridDim.y > 1 a share of the heads).  The loads of its first rows are on
-// their way while the table of slots is built; a group of lanes keeps four rows of bf16 (128 bytes a lane) in
-// flight.
-template <typename T, bool MXF, int TOKENS, int CHUNKS>
+// blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
+// (32 / group), all loads first; no warp waits for another.
+template <typename T, bool MXF, int CHUNKS, int ROWS>
 __global__ void __launch_bounds__(kThreads)
-kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, size_t tokens, long long n_slots,
-                int heads, int dim, int group, const FastDiv per_token, int wide, int32_t* status) {
-  constexpr int kInFlight = 8 / (int)sizeof(T) / CHUNKS;
-  __shared__ SlotTable<TOKENS> tab;
-  const size_t t0 = (size_t)blockIdx.x * TOKENS;
-  const int mine = (int)(tokens - t0 < (size_t)TOKENS ? tokens - t0 : (size_t)TOKENS);
-  const int per = (int)per_token.d / 2, h0 = blockIdx.y * per, here = min(per, heads - h0);  // heads of this CTA
-  const int lane = threadIdx.x & 31, sub = lane & (group - 1);
-  const int groups = kThreads / group, rows = mine * (int)per_token.d;  // (token, head, side)
-  const int r_first = (int)threadIdx.x / group;
-  Row<T, CHUNKS> x[kInFlight];
-  auto place = [&](int r, int& token, int& head, int& side) {
-    token = (int)per_token((uint32_t)r);
-    const int w = r - token * (int)per_token.d;
-    side = w & 1, head = w >> 1;
-    return r < rows && head < here;
-  };
-  auto load = [&](int r0) {
+kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, uint32_t tokens, long long n_slots,
+                const FastDiv by_heads, long long rows, int dim, int group_bits, const uint8_t* __restrict__ dead, int wide,
+                int32_t* status) {
+  const int lane = threadIdx.x & 31, group = 1 << group_bits, sub = lane & (group - 1);
+  const Side& sd = blockIdx.y ? v : k;
+  const int heads = (int)by_heads.d, across = 32 >> group_bits;
+  const long long r0 = ((long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (ROWS * across) + (lane >> group_bits);
+  pdl_wait();
+  pdl_launch_dependents();
+  Row<T, CHUNKS> x[ROWS];
+  long long slot[ROWS];
+  uint32_t token[ROWS];
+  int head[ROWS];
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      int token, head, side;
-      const bool ok = place(r0 + u * groups, token, head, side);
-      const Side& sd = side ? v : k;
-      x[u].load(reinterpret_cast<const T*>(sd.rows) + (long long)(t0 + token) * sd.token + (h0 + head) * sd.head, dim / 16, group, sub, ok, wide);
-    }
-  };
-  load(r_first);
-
-  constexpr uint32_t kSize = SlotTable<TOKENS>::kSize;
-  for (uint32_t i = threadIdx.x; i < kSize / 8; i += kThreads) reinterpret_cast<uint4*>(tab.head)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = threadIdx.x; i < mine; i += kThreads) {
-    long long s = index_at(slots, slot_bits, t0 + i);
-    if (s >= n_slots) {
-      s = -1;
-      if (status) atomicExch(status, (int)LQ_ERR_SHAPE);
-    }
-    tab.slot[i] = s < 0 ? -1 : s;
-    tab.dead[i] = 0;
+  for (int u = 0; u < ROWS; ++u) {
+    const long long r = r0 + u * across;
+    const bool ok = r < rows;
+    token[u] = ok ? by_heads((uint32_t)r) : 0;
+    head[u] = ok ? (int)((uint32_t)r - token[u] * heads) : 0;
+    x[u].load(reinterpret_cast<const T*>(sd.rows) + token[u] * sd.token + head[u] * sd.head, dim / 16, group, sub, ok, wide);
+    slot[u] = ok ? index_at(slots, slot_bits, token[u]) : -1;
+    if (dead && ok && __ldg(dead + token[u])) slot[u] = -1;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < mine; i += kThreads) {
-    const long long s = tab.slot[i];
-    if (s < 0) continue;
-    for (uint32_t h = slot_hash(s) % kSize;; h = (h + 1) % kSize) {
-      unsigned short old = atomicCAS(&tab.head[h], (unsigned short)0, (unsigned short)(i + 1));
-      if (old == 0) break;
-      if (tab.slot[old - 1] != s) continue;
-      // the entry stays with this slot: keep its latest token
-      while (old < i + 1) {
-        const unsigned short now = atomicCAS(&tab.head[h], old, (unsigned short)(i + 1));
-        if (now == old) break;
-        old = now;
-      }
-      tab.dead[old < i + 1 ? old - 1 : i] = 1;
-      break;
-    }
-  }
-  __syncthreads();
-  constexpr int kAhead = 4;
-  for (size_t t = t0 + TOKENS + threadIdx.x; t < tokens; t += kAhead * kThreads) {
-    long long s[kAhead];
+  if (!dead) {
+    // each lane keeps a share of all slots; every token among the warp's rows is compared with all of them
+    long long all[kInline / 32];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) s[j] = t + j * kThreads < tokens ? index_at(slots, slot_bits, t + j * kThreads) : -1;
+    for (int j = 0; j < kInline / 32; ++j) all[j] = lane + 32 * j < tokens ? index_at(slots, slot_bits, lane + 32 * j) : -1;
+    uint32_t last = 0xffffffffu;
+    bool again = false;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (s[j] < 0) continue;
-      for (uint32_t h = slot_hash(s[j]) % kSize;; h = (h + 1) % kSize) {
-        const int e = tab.head[h];
-        if (e == 0) break;
-        if (tab.slot[e - 1] == s[j]) {
-          tab.dead[e - 1] = 1;
-          break;
+    for (int u = 0; u < ROWS; ++u) {
+#pragma unroll 1
+      for (int i = 0; i < 32; i += group) {
+        const uint32_t t = __shfl_sync(0xffffffffu, token[u], i);
+        const long long s = __shfl_sync(0xffffffffu, slot[u], i);
+        if (t != last) {  // the same for the whole warp
+          again = false;
+#pragma unroll
+          for (int j = 0; j < kInline / 32; ++j) again |= all[j] == s && lane + 32 * j > t;
+          again = __any_sync(0xffffffffu, again);
+          last = t;
         }
+        if (again && lane >= i && lane < i + group) slot[u] = -1;
       }
     }
   }
-  __syncthreads();
-
-  for (int r0 = r_first; r0 - r_first < rows; r0 += kInFlight * groups) {
-    if (r0 != r_first) load(r0);
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      int token, head, side;
-      bool ok = place(r0 + u * groups, token, head, side);
-      const long long s = ok ? tab.slot[token] : -1;
-      ok = ok && s >= 0 && !tab.dead[token];
-      encode_row<T, MXF, CHUNKS>(side ? v : k, x[u], (size_t)(ok ? s : 0) * heads + h0 + head, dim, group, sub, ok);
+  for (int u = 0; u < ROWS; ++u) {
+    if (slot[u] >= n_slots) {
+      if (status) atomicExch(status, (int)LQ_ERR_SHAPE);
+      slot[u] = -1;
     }
+    const bool ok = slot[u] >= 0;
+    encode_row<T, MXF, CHUNKS>(sd, x[u], (size_t)(ok ? slot[u] : 0) * heads + head[u], dim, group, sub, ok);
   }
 }
 
@@ -269,6 +289,8 @@ __global__ void __launch_bounds__(kThreads)
 kv_read_kernel(const Side k, const Side v, const Table t, int heads, const FastDiv per_row, const FastDiv per_side,
                const FastDiv per_head, long long total, int clear_tail, int wide, int32_t* status) {
   const long long r0 = (((long long)blockIdx.x * kThreads + threadIdx.x) >> 5) * TOKENS;
+  pdl_wait();
+  pdl_launch_dependents();
   if (r0 >= total) return;
   const int lane = threadIdx.x & 31;
   const int rows = (int)(total - r0 < TOKENS ? total - r0 : TOKENS);
@@ -341,33 +363,35 @@ int check_format(const std::string& w, int format, size_t heads, size_t dim) {
   return LQ_OK;
 }
 
-template <typename T, bool MXF, int TOKENS, int CHUNKS>
-int write_tokens(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
-                 int dim, int group, int wide, int32_t* status, cudaStream_t st) {
-  const size_t tiles = (tokens + TOKENS - 1) / TOKENS;
-  if (tiles > 0x7fffffffu) return fail(LQ_ERR_SHAPE, "lq_kv_write: too many tokens for one launch");
-  // heads shared out until every SM has a CTA: a share repeats the table, but reads other rows
-  int per = heads;
-  while (per > 1 && tiles * (size_t)((heads + per - 1) / per) < 2 * (size_t)sm_count()) per = (per + 1) / 2;
-  kv_write_kernel<T, MXF, TOKENS, CHUNKS><<<dim3((unsigned)tiles, (unsigned)((heads + per - 1) / per)), kThreads, 0, st>>>(
-      k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, FastDiv(2 * (uint32_t)per), wide, status);
-  return check_cuda(cudaGetLastError(), "lq_kv_write launch");
+template <int TOKENS>
+int mark(const void* slots, int slot_bits, size_t tokens, uint8_t* dead, cudaStream_t st) {
+  return check_cuda(launch_pdl(kv_mark_kernel<TOKENS>, dim3((unsigned)((tokens + TOKENS - 1) / TOKENS)), dim3(kMarkThreads), 0, st, slots,
+                               slot_bits, tokens, dead),
+                    "lq_kv_write (mark) launch");
 }
 template <typename T, bool MXF, int CHUNKS>
-int write_chunks(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
-                 int dim, int group, int wide, int32_t* status, cudaStream_t st) {
-  // Every CTA looks at the slots of all later tokens, so its share of the tokens grows with their number.
-  if (tokens <= 8192) return write_tokens<T, MXF, 16, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
-  if (tokens <= 65536) return write_tokens<T, MXF, 64, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
-  return write_tokens<T, MXF, 256, CHUNKS>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+int write_rows(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads, int dim,
+               int group_bits, const uint8_t* dead, int wide, int32_t* status, cudaStream_t st) {
+  constexpr int ROWS = 8 / (int)sizeof(T) / CHUNKS;  // 128 bytes a lane in flight
+  const long long rows = (long long)tokens * heads, per_cta = (long long)(kThreads / 32) * ROWS * (32 >> group_bits);
+  return check_cuda(launch_pdl(kv_write_kernel<T, MXF, CHUNKS, ROWS>, dim3((unsigned)((rows + per_cta - 1) / per_cta), 2), dim3(kThreads), 0, st,
+                               k, v, slots, slot_bits, (uint32_t)tokens, n_slots, FastDiv((uint32_t)heads), rows, dim, group_bits, dead,
+                               wide, status),
+                    "lq_kv_write launch");
 }
 template <typename T, bool MXF>
 int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bits, size_t tokens, long long n_slots, int heads,
-                   int dim, int wide, int32_t* status, cudaStream_t st) {
-  int group = MXF ? 2 : 1;
-  while (group < 32 && group * 16 < dim) group *= 2;
-  if (dim <= 512) return write_chunks<T, MXF, 1>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
-  return write_chunks<T, MXF, 2>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group, wide, status, st);
+                   int dim, uint8_t* dead, int wide, int32_t* status, cudaStream_t st) {
+  int group_bits = MXF ? 1 : 0;
+  while (group_bits < 5 && (16 << group_bits) < dim) ++group_bits;
+  if (tokens > kInline) {
+    // few CTAs, each of which looks at the slots of all later tokens
+    if (int rc = tokens <= 16384 ? mark<128>(slots, slot_bits, tokens, dead, st) : mark<1024>(slots, slot_bits, tokens, dead, st)) return rc;
+  } else {
+    dead = nullptr;
+  }
+  if (dim <= 512) return write_rows<T, MXF, 1>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group_bits, dead, wide, status, st);
+  return write_rows<T, MXF, 2>(k, v, slots, slot_bits, tokens, n_slots, heads, dim, group_bits, dead, wide, status, st);
 }
 
 }  // namespace
@@ -375,14 +399,21 @@ int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bit
 
 using namespace lq;
 
+extern "C" size_t lq_kv_write_workspace_bytes(size_t tokens) { return tokens > (size_t)kInline ? tokens : 0; }
+
 extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t tokens, size_t heads, size_t dim, size_t k_token,
                            size_t k_head, size_t v_token, size_t v_head, const void* slots, int slot_bits, size_t n_slots, int format,
-                           void* k_codes, void* k_scales, void* v_codes, void* v_scales, int32_t* status, void* stream) {
+                           void* k_codes, void* k_scales, void* v_codes, void* v_scales, void* workspace, size_t workspace_bytes,
+                           int32_t* status, void* stream) {
   if (tokens == 0) return LQ_OK;
   if (!k || !v || !slots || !k_codes || !k_scales || !v_codes || !v_scales) return fail(LQ_ERR_DEVICE, "lq_kv_write: null pointer");
   if (in_dtype != LQ_F32 && in_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_kv_write: k and v must be f32|bf16");
   if (slot_bits != 32 && slot_bits != 64) return fail(LQ_ERR_DTYPE, "lq_kv_write: slots must be int32 or int64");
   if (int rc = check_format("lq_kv_write", format, heads, dim)) return rc;
+  // row numbers are 32-bit (2^31 rows of 16 values are 137 GB of float32)
+  if (tokens > 0x7fffffffu / heads) return fail(LQ_ERR_SHAPE, "lq_kv_write: tokens x heads must be below 2^31");
+  if (workspace_bytes < lq_kv_write_workspace_bytes(tokens) || (!workspace && tokens > (size_t)kInline))
+    return fail(LQ_ERR_WORKSPACE, "lq_kv_write: workspace too small");
   const size_t esz = in_dtype == LQ_F32 ? 4 : 2;
   if (!aligned16(k) || !aligned16(v) || (k_token * esz) % 16 || (k_head * esz) % 16 || (v_token * esz) % 16 || (v_head * esz) % 16)
     return fail(LQ_ERR_ALIGNMENT, "lq_kv_write: rows of k and v must be 16-byte aligned");
@@ -395,10 +426,10 @@ extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t to
   const int wide = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 32 == 0) &&
                    ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
   if (in_dtype == LQ_F32)
-    return format == LQ_KV_MXFP4 ? write_dispatch<float, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st)
-                                 : write_dispatch<float, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st);
-  return format == LQ_KV_MXFP4 ? write_dispatch<bf16, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st)
-                               : write_dispatch<bf16, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, wide, status, st);
+    return format == LQ_KV_MXFP4 ? write_dispatch<float, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, (uint8_t*)workspace, wide, status, st)
+                                 : write_dispatch<float, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, (uint8_t*)workspace, wide, status, st);
+  return format == LQ_KV_MXFP4 ? write_dispatch<bf16, true>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, (uint8_t*)workspace, wide, status, st)
+                               : write_dispatch<bf16, false>(ks, vs, slots, slot_bits, tokens, (long long)n_slots, h, d, (uint8_t*)workspace, wide, status, st);
 }
 
 extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int format,
@@ -430,9 +461,10 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   const size_t warps = few ? total : (total + 3) / 4;
   const unsigned grid = (unsigned)((warps * 32 + kThreads - 1) / kThreads);
   cudaStream_t st = (cudaStream_t)stream;
-#define LQ_KV_READ(T, F, N)                                                                                              \
-  kv_read_kernel<T, F, N><<<grid, kThreads, 0, st>>>(ks, vs, t, (int)heads, FastDiv(2 * side_chunks), FastDiv(side_chunks), \
-                                                     FastDiv(head_chunks), (long long)total, clear_tail, wide, status)
+  cudaError_t e;
+#define LQ_KV_READ(T, F, N)                                                                                         \
+  e = launch_pdl(kv_read_kernel<T, F, N>, dim3(grid), dim3(kThreads), 0, st, ks, vs, t, (int)heads, FastDiv(2 * side_chunks), \
+                 FastDiv(side_chunks), FastDiv(head_chunks), (long long)total, clear_tail, wide, status)
 #define LQ_KV_READ_T(T)                                     \
   if (format == LQ_KV_MXFP4) {                              \
     if (few) LQ_KV_READ(T, true, 1);                        \
@@ -448,5 +480,5 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   }
 #undef LQ_KV_READ_T
 #undef LQ_KV_READ
-  return check_cuda(cudaGetLastError(), "lq_kv_read launch");
+  return check_cuda(e, "lq_kv_read launch");
 }

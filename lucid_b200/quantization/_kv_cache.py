@@ -114,9 +114,12 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     kt, kh, _ = k.stride()
     vt, vh, _ = v.stride()
     kc, ks, vc, vs = cache
-    _lib.call("lq_kv_write", dev, k.data_ptr(), v.data_ptr(), _lib.code_of(k.dtype), shape[0], heads, dim, kt, kh, vt, vh,
+    tokens = shape[0]
+    room = tokens if tokens > 256 else 0  # lq_kv_write_workspace_bytes
+    ws = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
+    _lib.call("lq_kv_write", dev, k.data_ptr(), v.data_ptr(), _lib.code_of(k.dtype), tokens, heads, dim, kt, kh, vt, vh,
               slots.data_ptr(), 64 if slots.dtype == torch.int64 else 32, pages * page, fmt, kc.data_ptr(), ks.data_ptr(),
-              vc.data_ptr(), vs.data_ptr(), _lib.status_word(dev).data_ptr())
+              vc.data_ptr(), vs.data_ptr(), _addr(ws), room, _lib.status_word(dev).data_ptr())
 
 
 def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, total: int,

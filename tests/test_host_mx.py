@@ -56,7 +56,10 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.lq_mx_linear(*lin[:14], 16, *lin[15:]) == 6
     assert lib.lq_mx_linear(*lin[:13], None, *lin[14:]) == 3
     assert lib.lq_mx_linear(one, 5, *lin[2:]) == 2
-    kw = [one, one, 1, 4, 2, 64, 128, 64, 128, 64, one, 64, 32, 0, one, one, one, one, None, None]
+    kw = [one, one, 1, 4, 2, 64, 128, 64, 128, 64, one, 64, 32, 0, one, one, one, one, None, 0, None, None]
+    assert lib.lq_kv_write_workspace_bytes(256) == 0 and lib.lq_kv_write_workspace_bytes(257) == 257
+    assert lib.lq_kv_write(*kw[:3], 300, *kw[4:]) == 6
+    assert lib.lq_kv_write(*kw[:3], 1 << 31, *kw[4:]) == 1
     assert lib.lq_kv_write(None, None, 1, 0, *kw[4:]) == 0
     assert lib.lq_kv_write(None, *kw[1:]) == 3
     assert lib.lq_kv_write(*kw[:2], 4, *kw[3:]) == 2

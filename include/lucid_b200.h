@@ -492,7 +492,8 @@ int lq_mx_fake_quantize_grad(const void* grad, int dtype, const uint8_t* mask, s
 int lq_mx_matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes,
                  const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
                  int out_dtype, size_t ldo, int32_t* status, void* stream);
-/* lq_mx_quantize of x into the workspace, then lq_mx_matmul. */
+/* lq_mx_quantize of x into the workspace, then lq_mx_matmul; up to 16 rows in one launch without a
+ * workspace. */
 size_t lq_mx_linear_workspace_bytes(size_t M, size_t K);
 int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_t* w_codes,
                  const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,

@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "microscale.cuh"
 #include "tcgen05.cuh"
@@ -27,6 +28,9 @@ struct Args {
   int tiles_t, tiles_f;
   int split;             // CTAs (a cluster) that share the K axis of a tile
   int early;             // the weight may be fetched before the preceding kernel has finished
+  const void* x;         // activations to encode on the way (fused form): row stride, 32-byte loads, columns
+  long long ldx;
+  int x_wide, K;
   const float* bias;
   int relu;
   void* out;
@@ -171,7 +175,10 @@ struct Cfg {
   static_assert(TN * kRows * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
 };
 
-template <int TN, typename T>
+// With X other than void the activations are still float32 or bf16: the epilogue warps, idle until the product
+// is done, encode them stage by stage into the places where TMA would have put codes and scales (every CTA of
+// a layer repeats that for its part of K: a few KB of a few tokens).  One launch instead of two.
+template <int TN, typename T, typename X = void>
 __global__ void __launch_bounds__(kThreads, 2)
 mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                const __grid_constant__ CUtensorMap tm_sw, const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ Args g) {
@@ -191,9 +198,11 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   const int kb0 = (int)((long long)g.num_kb * rank / g.split), kb1 = (int)((long long)g.num_kb * (rank + 1) / g.split);
   const int n = kb1 - kb0;
   const uint32_t smem0 = smem_u32(smem);
+  constexpr bool kFused = !std::is_same<X, void>::value;
+  constexpr int kEncodeWarps = 4;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2 * C::kStages + 1; ++s) mbar_init(bar_full + 8 * s, 1);
+    for (int s = 0; s < 2 * C::kStages + 1; ++s) mbar_init(bar_full + 8 * s, kFused && s < C::kStages ? 1 + kEncodeWarps : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
@@ -212,7 +221,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   if (warp == 0) {
     auto load_w = [&](int i, int s) {
       const uint32_t dst = smem0 + s * C::kStageBytes, bar = bar_full + 8 * s;
-      mbar_expect_tx(bar, C::kStageBytes);
+      mbar_expect_tx(bar, kFused ? kWBytes + mx::kTileBytes : C::kStageBytes);
       tma_load_2d(dst, &tm_w, (kb0 + i) * 128, f0, bar);
       tma_load_3d(dst + kWBytes + C::kXBytes, &tm_sw, 0, kb0 + i, f0 / mx::kTileRows, bar);
     };
@@ -229,9 +238,11 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
       if (!mbar_wait_warp(bar_empty + 8 * s, phase, abort_flag, g.budget)) break;
       if (elect_one()) {
         if (i >= pre) load_w(i, s);
-        const uint32_t dst = smem0 + s * C::kStageBytes, bar = bar_full + 8 * s;
-        tma_load_2d(dst + kWBytes, &tm_x, (kb0 + i) * 128, t0, bar);
-        tma_load_3d(dst + kWBytes + C::kXBytes + mx::kTileBytes, &tm_sx, 0, kb0 + i, t0 / mx::kTileRows, bar);
+        if (!kFused) {
+          const uint32_t dst = smem0 + s * C::kStageBytes, bar = bar_full + 8 * s;
+          tma_load_2d(dst + kWBytes, &tm_x, (kb0 + i) * 128, t0, bar);
+          tma_load_3d(dst + kWBytes + C::kXBytes + mx::kTileBytes, &tm_sx, 0, kb0 + i, t0 / mx::kTileRows, bar);
+        }
       }
       if (++s == C::kStages) s = 0, phase ^= 1;
     }
@@ -271,8 +282,60 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   const bool epilogue = warp >= 2;
   const int quad = warp & 3;
   bool ok = true;
+  if constexpr (kFused) {
+    static_assert(TN == 16, "one scale tile, two swizzle atoms of tokens");
+    if (epilogue) {
+      pdl_wait();
+      const int tid = (int)threadIdx.x - 64;
+      // a thread encodes chunk c of sixteen values of row r and of row r + 8
+      const int c = tid & 15, r = tid >> 4;
+      const bool high = g.M > 8;
+      const X* x = reinterpret_cast<const X*>(g.x) + r * g.ldx + c * 16;
+      mx::Chunk<X> v[2];
+      auto fetch = [&](int i) {
+        const int k = (kb0 + i) * kStageK;
+        const bool in_k = k + c * 16 < g.K;
+        if (in_k && r < g.M) v[0].load(x + k, g.x_wide);
+        else v[0].clear();
+        if (in_k && r + 8 < g.M) v[1].load(x + 8 * g.ldx + k, g.x_wide);
+        else v[1].clear();
+      };
+      // row r of the swizzled tile: 16-byte piece p lies at piece p ^ (r % 8); rows 8.. are the next 1024 bytes
+      const int code_at = kWBytes + r * 128 + (((c >> 1) ^ r) << 4) + (c & 1) * 8;
+      const int scale_at = kWBytes + C::kXBytes + mx::kTileBytes + mx::tile_offset(r, c >> 1);
+      fetch(0);
+      // rows past the last token stay zero
+      constexpr int kPieces = (C::kXBytes + mx::kTileBytes) / 16;
+      for (int i = tid; i < C::kStages * kPieces; i += 32 * kEncodeWarps) {
+        const int s = i / kPieces, o = (i - s * kPieces) * 16;
+        const int at = o < C::kXBytes ? kWBytes + o : kWBytes + mx::kTileBytes + o;  // codes, then (past the weight's) scales
+        *reinterpret_cast<uint4*>(smem + s * C::kStageBytes + at) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      int s = 0;
+      uint32_t phase = 1;
+      for (int i = 0; i < n; ++i) {
+        if (!mbar_wait_warp(bar_empty + 8 * s, phase, abort_flag, g.budget)) break;
+        uint8_t* stage = smem + s * C::kStageBytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && !high) break;
+          const uint32_t byte = mx::block_byte<X>(v[h]);
+          if (r + 8 * h < g.M) {
+            *reinterpret_cast<uint2*>(stage + code_at + h * 1024) = mx::encode16<X>(v[h], byte);
+            if (!(c & 1)) stage[scale_at + h * 8 * 16] = (uint8_t)byte;
+          }
+        }
+        if (i + 1 < n) fetch(i + 1);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what these stores wrote
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_full + 8 * s);
+        if (++s == C::kStages) s = 0, phase ^= 1;
+      }
+    }
+  }
   if (epilogue) {
-    pdl_wait();
+    if (!kFused) pdl_wait();
     ok = mbar_wait_warp(bar_done, 0, abort_flag, g.budget);
     tc_fence_after();
   }
@@ -548,6 +611,7 @@ EncodeFn get_encode() {
 }
 // codes: (rows, K / 2) bytes, boxes of 128 bytes x box_rows, rows and bytes past the end read as zeros
 int code_map(CUtensorMap* tm, const void* base, size_t rows, size_t K, int box_rows) {
+  if (!get_encode()) return fail(LQ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
   const cuuint64_t dims[2] = {K / 2, rows}, strides[1] = {K / 2};
   const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, ones[2] = {1, 1};
   const CUresult r = get_encode()(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones,
@@ -557,6 +621,7 @@ int code_map(CUtensorMap* tm, const void* base, size_t rows, size_t K, int box_r
 }
 // scale tiles: (row tiles, column tiles, 256 words), boxes of one column tile x box_tiles row tiles
 int scale_map(CUtensorMap* tm, const void* base, size_t rows, size_t K, int box_tiles) {
+  if (!get_encode()) return fail(LQ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
   const cuuint64_t ct = (K + kStageK - 1) / kStageK, rt = (rows + mx::kTileRows - 1) / mx::kTileRows;
   const cuuint64_t dims[3] = {256, ct, rt}, strides[2] = {mx::kTileBytes, ct * mx::kTileBytes};
   const cuuint32_t box[3] = {256, 1, (cuuint32_t)box_tiles}, ones[3] = {1, 1, 1};
@@ -570,12 +635,13 @@ struct Operands {
   const uint8_t *x, *sx, *w, *sw;
   size_t M, N, K;
 };
+constexpr size_t kFusedTokens = 16;
 
-template <int TN, typename T>
+template <int TN, typename T, typename X = void>
 int launch_tile(const Operands& o, Args g, cudaStream_t st) {
   static PerDeviceOnce once;
   using C = Cfg<TN>;
-  auto kernel = mx_tile_kernel<TN, T>;
+  auto kernel = mx_tile_kernel<TN, T, X>;
   const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); });
   if (e != cudaSuccess) return check_cuda(e, "cudaFuncSetAttribute(max dynamic smem)");
   g.tiles_t = (g.M + TN - 1) / TN, g.tiles_f = (g.N + kRows - 1) / kRows;
@@ -591,9 +657,13 @@ int launch_tile(const Operands& o, Args g, cudaStream_t st) {
   if (tiles * g.split > 0x7fffffffll) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: too many tiles for one launch");
   CUtensorMap tw, tx, tsw, tsx;
   if (int rc = code_map(&tw, o.w, o.N, o.K, kRows)) return rc;
-  if (int rc = code_map(&tx, o.x, o.M, o.K, TN)) return rc;
   if (int rc = scale_map(&tsw, o.sw, o.N, o.K, 1)) return rc;
-  if (int rc = scale_map(&tsx, o.sx, o.M, o.K, 1)) return rc;
+  if (std::is_same<X, void>::value) {
+    if (int rc = code_map(&tx, o.x, o.M, o.K, TN)) return rc;
+    if (int rc = scale_map(&tsx, o.sx, o.M, o.K, 1)) return rc;
+  } else {
+    tx = tw, tsx = tsw;  // not used
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * g.split)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = C::kSmemBytes, cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -655,26 +725,29 @@ int launch(const Operands& o, const Args& g, cudaStream_t st) {
   return launch_pair<T>(o, g, st);
 }
 
-int matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes, const uint8_t* w_scales, size_t N, size_t K,
-           const float* bias, int relu, void* out, int out_dtype, size_t ldo, int32_t* status, int early, cudaStream_t st) {
-  if (!a_codes || !a_scales || !w_codes || !w_scales || !out) return fail(LQ_ERR_DEVICE, "lq_mx_matmul: null pointer");
-  if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_mx_matmul: out must be f32|bf16");
-  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: K must be a multiple of 32");
-  if (M >= ((size_t)1 << 30) || N >= ((size_t)1 << 30) || K >= ((size_t)1 << 30)) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: extents must be below 2^30");
-  if (ldo < N) return fail(LQ_ERR_SHAPE, "lq_mx_matmul: output row stride shorter than a row");
-  if (!aligned16(a_codes) || !aligned16(a_scales) || !aligned16(w_codes) || !aligned16(w_scales))
-    return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: codes and scales must be 16-byte aligned");
+// What every form of the product asks of its weight, result and extents; fills the common arguments.
+int prepare(const char* who, Args* g, size_t M, const uint8_t* w_codes, const uint8_t* w_scales, size_t N, size_t K, const float* bias,
+            int relu, void* out, int out_dtype, size_t ldo, int32_t* status) {
+  const std::string w(who);
+  if (!w_codes || !w_scales || !out) return fail(LQ_ERR_DEVICE, w + ": null pointer");
+  if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, w + ": out must be f32|bf16");
+  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, w + ": K must be a multiple of 32");
+  if (M >= ((size_t)1 << 30) || N >= ((size_t)1 << 30) || K >= ((size_t)1 << 30)) return fail(LQ_ERR_SHAPE, w + ": extents must be below 2^30");
+  if (ldo < N) return fail(LQ_ERR_SHAPE, w + ": output row stride shorter than a row");
   const size_t esz = out_dtype == LQ_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(out) % esz != 0) return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: out must be aligned to its type");
-  if (!get_encode()) return fail(LQ_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
-  Args g;
-  memset(&g, 0, sizeof(g));
-  g.M = (int)M, g.N = (int)N, g.num_kb = (int)((K + kStageK - 1) / kStageK);
-  g.early = early, g.bias = bias, g.relu = relu, g.out = out, g.ldo = (long long)ldo, g.status = status, g.budget = kWaitBudgetCycles;
-  g.pairs_ok = out_dtype == LQ_BF16 && reinterpret_cast<uintptr_t>(out) % 4 == 0 && ldo % 2 == 0 && N % 2 == 0;
-  g.quads_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
-  const Operands o = {a_codes, a_scales, w_codes, w_scales, M, N, K};
-  return out_dtype == LQ_F32 ? launch<float>(o, g, st) : launch<__nv_bfloat16>(o, g, st);
+  if (!aligned16(w_codes) || !aligned16(w_scales) || reinterpret_cast<uintptr_t>(out) % esz != 0)
+    return fail(LQ_ERR_ALIGNMENT, w + ": codes and scales must be 16-byte aligned, out to its type");
+  memset(g, 0, sizeof(*g));
+  g->M = (int)M, g->N = (int)N, g->K = (int)K, g->num_kb = (int)((K + kStageK - 1) / kStageK);
+  g->bias = bias, g->relu = relu, g->out = out, g->ldo = (long long)ldo, g->status = status, g->budget = kWaitBudgetCycles;
+  g->pairs_ok = out_dtype == LQ_BF16 && reinterpret_cast<uintptr_t>(out) % 4 == 0 && ldo % 2 == 0 && N % 2 == 0;
+  g->quads_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
+  return LQ_OK;
+}
+
+template <typename T>
+int launch_fused(const Operands& o, const Args& g, int in_dtype, cudaStream_t st) {
+  return in_dtype == LQ_F32 ? launch_tile<16, T, float>(o, g, st) : launch_tile<16, T, __nv_bfloat16>(o, g, st);
 }
 
 }  // namespace
@@ -683,24 +756,45 @@ int matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint
 using namespace lq;
 
 extern "C" size_t lq_mx_linear_workspace_bytes(size_t M, size_t K) {
-  return (M * (K / 2) + 1023) / 1024 * 1024 + lq_mx_scale_bytes(M, K);
+  return M <= kFusedTokens ? 0 : (M * (K / 2) + 1023) / 1024 * 1024 + lq_mx_scale_bytes(M, K);
 }
 
 extern "C" int lq_mx_matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes,
                             const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
                             int out_dtype, size_t ldo, int32_t* status, void* stream) {
   if (M == 0 || N == 0) return LQ_OK;
-  return matmul(a_codes, a_scales, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status, 0, (cudaStream_t)stream);
+  if (!a_codes || !a_scales) return fail(LQ_ERR_DEVICE, "lq_mx_matmul: null pointer");
+  Args g;
+  if (int rc = prepare("lq_mx_matmul", &g, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status)) return rc;
+  if (!aligned16(a_codes) || !aligned16(a_scales)) return fail(LQ_ERR_ALIGNMENT, "lq_mx_matmul: codes and scales must be 16-byte aligned");
+  const Operands o = {a_codes, a_scales, w_codes, w_scales, M, N, K};
+  cudaStream_t st = (cudaStream_t)stream;
+  return out_dtype == LQ_F32 ? launch<float>(o, g, st) : launch<__nv_bfloat16>(o, g, st);
 }
 
 extern "C" int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
                             size_t N, size_t K, const float* bias, int relu, void* out, int out_dtype, size_t ldo,
                             uint8_t* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   if (M == 0 || N == 0) return LQ_OK;
+  Args g;
+  if (int rc = prepare("lq_mx_linear", &g, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  Operands o = {nullptr, nullptr, w_codes, w_scales, M, N, K};
+  if (M <= kFusedTokens) {
+    if (!x) return fail(LQ_ERR_DEVICE, "lq_mx_linear: null pointer");
+    if (in_dtype != LQ_F32 && in_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_mx_linear: x must be f32|bf16");
+    const size_t esz = in_dtype == LQ_F32 ? 4 : 2;
+    if (ldx < K) return fail(LQ_ERR_SHAPE, "lq_mx_linear: row stride shorter than a row");
+    if (!aligned16(x) || (ldx * esz) % 16 != 0) return fail(LQ_ERR_ALIGNMENT, "lq_mx_linear: rows of x must be 16-byte aligned");
+    g.x = x, g.ldx = (long long)ldx, g.x_wide = reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * esz) % 32 == 0;
+    return out_dtype == LQ_F32 ? launch_fused<float>(o, g, in_dtype, st) : launch_fused<__nv_bfloat16>(o, g, in_dtype, st);
+  }
   if (!workspace) return fail(LQ_ERR_DEVICE, "lq_mx_linear: null workspace");
-  if (K == 0 || K % mx::kBlock != 0) return fail(LQ_ERR_SHAPE, "lq_mx_linear: K must be a multiple of 32");
+  if (!aligned16(workspace)) return fail(LQ_ERR_ALIGNMENT, "lq_mx_linear: the workspace must be 16-byte aligned");
   if (workspace_bytes < lq_mx_linear_workspace_bytes(M, K)) return fail(LQ_ERR_WORKSPACE, "lq_mx_linear: workspace too small");
   uint8_t* a_scales = workspace + (M * (K / 2) + 1023) / 1024 * 1024;
   if (int rc = lq_mx_quantize(x, in_dtype, M, K, ldx, workspace, a_scales, stream)) return rc;
-  return matmul(workspace, a_scales, M, w_codes, w_scales, N, K, bias, relu, out, out_dtype, ldo, status, 1, (cudaStream_t)stream);
+  g.early = 1;
+  o.x = workspace, o.sx = a_scales;
+  return out_dtype == LQ_F32 ? launch<float>(o, g, st) : launch<__nv_bfloat16>(o, g, st);
 }

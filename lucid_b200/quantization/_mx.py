@@ -201,9 +201,10 @@ def mx_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bi
     b = _bias_of(bias, n, dev)
     x2, m, _, ld = _rows(x)
     out = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
-    room = (m * (k // 2) + 1023) // 1024 * 1024 + (m + 127) // 128 * ((k + 255) // 256) * 1024
-    ws = torch.empty(room, dtype=torch.uint8, device=dev)
+    # lq_mx_linear_workspace_bytes
+    room = 0 if m <= 16 else (m * (k // 2) + 1023) // 1024 * 1024 + (m + 127) // 128 * ((k + 255) // 256) * 1024
+    ws = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
     code = _lib.code_of(x.dtype)
     _lib.call("lq_mx_linear", dev, x2.data_ptr(), code, m, ld, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
-              int(relu), out.data_ptr(), code, n, ws.data_ptr(), room, _lib.status_word(dev).data_ptr())
+              int(relu), out.data_ptr(), code, n, _addr(ws), room, _lib.status_word(dev).data_ptr())
     return out

@@ -189,7 +189,8 @@ def test_relu_keeps_nan():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("lead,k,n", [((1,), 2048, 512), ((3, 5), 96, 40), ((130,), 1056, 1003), ((2, 1, 40), 512, 8)])
+@pytest.mark.parametrize("lead,k,n", [((1,), 2048, 512), ((1,), 32, 8), ((3, 5), 96, 40), ((8,), 8192, 130), ((9,), 1312, 257),
+                                      ((16,), 4096, 384), ((17,), 4096, 384), ((130,), 1056, 1003), ((2, 1, 40), 512, 8)])
 def test_linear_is_quantize_and_product(lead, k, n, dtype):
     rng = np.random.default_rng(k + n)
     x = _sample(rng, int(np.prod(lead)), k, dtype).reshape(*lead, k).cuda()
@@ -200,6 +201,12 @@ def test_linear_is_quantize_and_product(lead, k, n, dtype):
     assert torch.equal(y, Q.mx_matmul(*Q.mx_quantize(x), *w, bias=bias, relu=True, out_dtype=dtype))
     strided = torch.cat((x, x), -1)[..., :k]
     assert torch.equal(Q.mx_linear(strided, *w, bias=bias, relu=True), y)
+    apart = torch.empty(*lead, k + 24, dtype=dtype, device="cuda")[..., 8:8 + k]  # 16-byte, not 32-byte aligned rows of bf16
+    apart.copy_(x)
+    assert torch.equal(Q.mx_linear(apart, *w, bias=bias, relu=True), y)
+    poisoned = x.clone()
+    poisoned.view(-1, k)[0, k - 1] = float("inf")
+    assert torch.isnan(Q.mx_linear(poisoned, *w).view(-1, n)[0]).all()
 
 
 def test_layer_state_dict_and_workflows():

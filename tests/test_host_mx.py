@@ -29,7 +29,7 @@ def test_c_entries_refuse_without_a_gpu():
     lib = _lib.load()
     one, odd = ctypes.c_void_p(16), ctypes.c_void_p(8)
     assert lib.lq_mx_scale_bytes(1, 32) == 1024 and lib.lq_mx_scale_bytes(129, 257) == 4096 and lib.lq_mx_scale_bytes(0, 64) == 0
-    assert lib.lq_mx_linear_workspace_bytes(3, 64) == 1024 + 1024
+    assert lib.lq_mx_linear_workspace_bytes(16, 64) == 0 and lib.lq_mx_linear_workspace_bytes(17, 64) == 1024 + 1024
     q = [one, 0, 4, 64, 64, one, one, None]
     assert lib.lq_mx_quantize(None, 0, 0, 64, 64, None, None, None) == 0  # nothing to do
     assert lib.lq_mx_quantize(None, *q[1:]) == 3
@@ -52,10 +52,12 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.lq_mx_matmul(*mm[:11], 7, *mm[12:]) == 1
     assert lib.lq_mx_matmul(odd, *mm[1:]) == 4
     assert lib.lq_mx_matmul(*mm[:2], 1 << 40, *mm[3:]) == 1
-    lin = [one, 0, 4, 64, one, one, 8, 64, None, 0, one, 0, 8, one, 1 << 20, None, None]
+    lin = [one, 0, 20, 64, one, one, 8, 64, None, 0, one, 0, 8, one, 1 << 20, None, None]
     assert lib.lq_mx_linear(*lin[:14], 16, *lin[15:]) == 6
     assert lib.lq_mx_linear(*lin[:13], None, *lin[14:]) == 3
-    assert lib.lq_mx_linear(one, 5, *lin[2:]) == 2
+    assert lib.lq_mx_linear(one, 5, *lin[2:]) == 2 and lib.lq_mx_linear(one, 5, 4, *lin[3:]) == 2
+    assert lib.lq_mx_linear(None, 0, 4, *lin[3:]) == 3 and lib.lq_mx_linear(odd, 0, 4, *lin[3:]) == 4
+    assert lib.lq_mx_linear(one, 0, 4, 32, *lin[4:]) == 1 and lib.lq_mx_linear(one, 0, 4, 66, *lin[4:]) == 4
     kw = [one, one, 1, 4, 2, 64, 128, 64, 128, 64, one, 64, 32, 0, one, one, one, one, None, 0, None, None]
     assert lib.lq_kv_write_workspace_bytes(256) == 0 and lib.lq_kv_write_workspace_bytes(257) == 257
     assert lib.lq_kv_write(*kw[:3], 300, *kw[4:]) == 6

@@ -352,6 +352,17 @@ def status_word(device: torch.device) -> torch.Tensor:
     return w
 
 
+def status_ptr(device: torch.device):
+    """Address of the status word, or None inside a capture that comes before its first use (a word
+    made there would belong to the graph's memory, and every replay would clear it)."""
+    w = _status_words.get(device.index)
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        w = status_word(device)
+    return w.data_ptr()
+
+
 def check_device_status(device: torch.device) -> None:
     """Synchronising check of what the kernels report from the device: the status word of the
     contraction / exchange kernels and the give-up count of the pipelined stream kernels.  Raises

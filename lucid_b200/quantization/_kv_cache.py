@@ -119,7 +119,7 @@ def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     ws = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
     _lib.call("lq_kv_write", dev, k.data_ptr(), v.data_ptr(), _lib.code_of(k.dtype), tokens, heads, dim, kt, kh, vt, vh,
               slots.data_ptr(), 64 if slots.dtype == torch.int64 else 32, pages * page, fmt, kc.data_ptr(), ks.data_ptr(),
-              vc.data_ptr(), vs.data_ptr(), _addr(ws), room, _lib.status_word(dev).data_ptr())
+              vc.data_ptr(), vs.data_ptr(), _addr(ws), room, _lib.status_ptr(dev))
 
 
 def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -181,5 +181,5 @@ def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.
     kc, ks, vc, vs = cache
     _lib.call("lq_kv_read", dev, kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), fmt, pages, page, heads, dim,
               table.data_ptr(), table.stride(0), max_blocks, cu.data_ptr(), _addr(starts), seqs, total, ok.data_ptr(),
-              ov.data_ptr(), _lib.code_of(ok.dtype), kt, kh, vt, vh, int(out is None), _lib.status_word(dev).data_ptr())
+              ov.data_ptr(), _lib.code_of(ok.dtype), kt, kh, vt, vh, int(out is None), _lib.status_ptr(dev))
     return ok, ov

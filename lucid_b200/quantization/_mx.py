@@ -182,7 +182,7 @@ def mx_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tens
     b = _bias_of(bias, n, dev)
     out = torch.empty(*a_codes.shape[:-1], n, dtype=out_dtype, device=dev)
     _lib.call("lq_mx_matmul", dev, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
-              int(relu), out.data_ptr(), _lib.code_of(out_dtype), n, _lib.status_word(dev).data_ptr())
+              int(relu), out.data_ptr(), _lib.code_of(out_dtype), n, _lib.status_ptr(dev))
     return out
 
 
@@ -206,5 +206,5 @@ def mx_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bi
     ws = torch.empty(room, dtype=torch.uint8, device=dev) if room else None
     code = _lib.code_of(x.dtype)
     _lib.call("lq_mx_linear", dev, x2.data_ptr(), code, m, ld, wc.data_ptr(), sw.data_ptr(), n, k, _addr(b),
-              int(relu), out.data_ptr(), code, n, _addr(ws), room, _lib.status_word(dev).data_ptr())
+              int(relu), out.data_ptr(), code, n, _addr(ws), room, _lib.status_ptr(dev))
     return out

@@ -141,7 +141,9 @@ def _to_device(code, byte):
 
 SHAPES = [(1, 32, 16), (1, 64, 1), (1, 8192, 300), (2, 96, 128), (5, 256, 129), (8, 320, 200), (9, 288, 1000), (16, 4096, 256),
           (17, 512, 384), (33, 1056, 130), (64, 992, 520), (65, 2048, 257), (100, 4096, 640), (128, 256, 128), (129, 1056, 1003),
-          (200, 64, 72), (256, 512, 256), (257, 736, 515), (300, 32, 2000), (777, 1056, 1003), (1024, 2048, 1024)]
+          (200, 64, 72), (256, 512, 256), (257, 736, 515), (300, 32, 2000), (777, 1056, 1003), (1024, 2048, 1024),
+          # tiles of 128 tokens, then CTA pairs: few and many stages, several tiles to a pair, ragged ends
+          (1000, 352, 4096), (1300, 800, 4100), (2050, 32, 2561), (700, 4224, 8200), (129, 1312, 20001), (3000, 2048, 2600)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
@@ -181,6 +183,21 @@ def test_products_with_nan_blocks_and_extreme_scales():
     assert np.isnan(y[3]).all() and np.isnan(y[:, 140]).all()
     keep = ~np.isnan(ref)
     assert np.array_equal(np.isnan(y), ~keep) and np.array_equal(y[keep], ref[keep].astype(np.float32))
+
+
+@pytest.mark.parametrize("m,n", [(3, 300), (70, 300), (1300, 4100), (1000, 4096)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_the_result_may_lie_apart(m, n, dtype):
+    """The C entry's row stride: columns past N and rows past M stay as they were."""
+    rng = np.random.default_rng(m)
+    a, w = _grid(rng, m, 288, 0), _grid(rng, n, 288, 0)
+    ac, sa, wc, sw = *_to_device(*a), *_to_device(*w)
+    ref = torch.from_numpy((MX.decode(*a) @ MX.decode(*w).T).astype(np.float32)).to(dtype)
+    for ldo in (n + 5, n + 8):
+        out = torch.full((m + 2, ldo), -7.0, dtype=dtype, device="cuda")
+        _lib.call("lq_mx_matmul", out.device, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, 288, None, 0,
+                  out.data_ptr(), _lib.code_of(dtype), ldo, None)
+        assert torch.equal(out[:m, :n].cpu(), ref) and (out[:m, n:] == -7.0).all() and (out[m:] == -7.0).all()
 
 
 def test_relu_keeps_nan():
@@ -271,9 +288,40 @@ def test_captured_and_replayed():
         assert torch.equal(y, Q.mx_linear(x, *w))
 
 
-def test_two_streams_at_once():
-    ws = [Q.mx_quantize(torch.randn(640, 2048, device="cuda")) for _ in range(2)]
-    xs = [torch.randn(96, 2048, device="cuda") for _ in range(2)]
+def test_captured_before_anything_else(monkeypatch):
+    """A capture that is the first use makes no status word inside the graph's memory."""
+    monkeypatch.setattr(_lib, "_status_words", {})
+    x, w = torch.randn(4, 64, device="cuda"), Q.mx_quantize(torch.randn(8, 64, device="cuda"))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = Q.mx_linear(x, *w)
+    assert _lib._status_words == {}
+    graph.replay()
+    assert torch.equal(y, Q.mx_linear(x, *w))
+
+
+def test_training_step_captured_and_replayed():
+    """(With no eager graph of the leaf alive: torch ties a leaf's gradient node to the stream of its first
+    use, and refuses to capture a backward pass of any operator through a node of another stream.)"""
+    leaf = torch.randn(64, 96, device="cuda", requires_grad=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(Q.mx_fake_quantize(leaf).sum(), leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (g,) = torch.autograd.grad(Q.mx_fake_quantize(leaf).sum(), leaf)
+    with torch.no_grad():
+        leaf.copy_(torch.randn(64, 96, device="cuda") * 3)
+    graph.replay()
+    assert np.array_equal(host(g), MX.encode(host(leaf.detach()))[2].astype(np.float32))
+
+
+@pytest.mark.parametrize("rows,width", [(96, 640), (1300, 4100)])
+def test_two_streams_at_once(rows, width):
+    ws = [Q.mx_quantize(torch.randn(width, 2048, device="cuda")) for _ in range(2)]
+    xs = [torch.randn(rows, 2048, device="cuda") for _ in range(2)]
     want = [Q.mx_linear(x, *w) for x, w in zip(xs, ws)]
     torch.cuda.synchronize()
     streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]

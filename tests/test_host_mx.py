@@ -131,6 +131,7 @@ def test_workflows_route_the_linear_family(monkeypatch):
         backends.quantized.engine = "mxfp8"
     abi_standin.install(monkeypatch, engine="mxfp4")
     monkeypatch.setattr(_lib, "call", _numpy_call)
+    monkeypatch.setattr(_lib, "status_ptr", lambda device: None)
     assert backends.quantized.use_mx() and not backends.quantized.use_mlx() and not backends.quantized.use_int8()
     torch.manual_seed(1)
     net = torch.nn.Sequential(torch.nn.Linear(96, 160), torch.nn.ReLU(), torch.nn.Linear(160, 48), torch.nn.Linear(48, 8)).eval()

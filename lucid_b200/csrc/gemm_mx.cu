@@ -345,7 +345,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   if (g.split == 1) {
     if (epilogue && ok) {
       const int f = f0 + quad * 32 + lane;
-      const float b = g.bias && f < g.N ? __ldg(g.bias + f) : 0.0f;
+      const float b = g.bias && f < g.N ? __ldcg(g.bias + f) : 0.0f;
 #pragma unroll 1
       for (int c = 0; c < valid; c += 16) {
         uint32_t r[16];
@@ -385,7 +385,7 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         if (r < g.split) v[0] = __fadd_rn(v[0], p[r].x), v[1] = __fadd_rn(v[1], p[r].y), v[2] = __fadd_rn(v[2], p[r].z), v[3] = __fadd_rn(v[3], p[r].w);
       if (*abort_flag != 0) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = finish(v[j], g.bias && f + j < g.N ? __ldg(g.bias + f + j) : 0.0f, g.bias != nullptr, g.relu);
+      for (int j = 0; j < 4; ++j) v[j] = finish(v[j], g.bias && f + j < g.N ? __ldcg(g.bias + f + j) : 0.0f, g.bias != nullptr, g.relu);
       store4(reinterpret_cast<T*>(g.out) + (long long)t * g.ldo + f, v, g.N - f, g.quads_ok);
     }
     cluster_sync_all();  // nobody's partial sums go away while they are read
@@ -546,7 +546,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
       const int t0 = tile % g.tiles_t * kPairTokens;
       const int f = tile / g.tiles_t * 2 * kRows + (int)rank * kRows + quad * 32 + lane;
       const int acc = q & 1;
-      const float b = g.bias && f < g.N ? __ldg(g.bias + f) : 0.0f;
+      const float b = g.bias && f < g.N ? __ldcg(g.bias + f) : 0.0f;
       if (!mbar_wait_warp(bar_tfull + 8 * acc, (q >> 1) & 1, abort_flag, g.budget)) break;
       tc_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + acc * kAccStep;

@@ -23,8 +23,34 @@ struct Side {           // keys or values
   void* rows;           // new rows (write), output rows (read)
   long long token, head;  // their strides
 };
+// Plain loads (through L1, not the read-only path: see load_once) of what a few lanes or warps share.
+__device__ __forceinline__ int load_common(const int* p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ long long load_common(const long long* p) {
+  long long v;
+  asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float load_common(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_common(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 load_common(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ long long index_at(const void* p, int bits, size_t i) {
-  return bits == 64 ? __ldg(reinterpret_cast<const long long*>(p) + i) : (long long)__ldg(reinterpret_cast<const int*>(p) + i);
+  return bits == 64 ? load_common(reinterpret_cast<const long long*>(p) + i) : (long long)load_common(reinterpret_cast<const int*>(p) + i);
 }
 
 // n / d for n * d < 2^43 (the rounding of m adds less than d * n / 2^43 < 1 / d to the quotient), n < 2^31, by the
@@ -283,21 +309,21 @@ struct Table {
 
 // Slot of output row r, -1 where the table has none for it; `covered` says whether a sequence has the row.
 __device__ __forceinline__ long long find_slot(const Table& t, long long r, bool& covered) {
-  covered = r < (long long)__ldg(t.cu + t.seqs) && r >= (long long)__ldg(t.cu);
+  covered = r < (long long)load_common(t.cu + t.seqs) && r >= (long long)load_common(t.cu);
   if (!covered) return -1;
   int lo = 0, hi = t.seqs;  // the first index with cu[index] > r
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if ((long long)__ldg(t.cu + mid) > r) hi = mid;
+    if ((long long)load_common(t.cu + mid) > r) hi = mid;
     else lo = mid + 1;
   }
   if (lo == 0) return -1;  // cu does not ascend
   const int b = lo - 1;
-  const long long pos = r - __ldg(t.cu + b) + (t.starts ? __ldg(t.starts + b) : 0);
+  const long long pos = r - load_common(t.cu + b) + (t.starts ? load_common(t.starts + b) : 0);
   if (pos < 0 || pos > 0x7fffffffll) return -1;
   const int blk = (int)pos / t.page;
   if (blk >= t.max_blocks) return -1;
-  const long long p = __ldg(t.pages + b * t.stride + blk);
+  const long long p = load_common(t.pages + b * t.stride + blk);
   return p < 0 || p >= t.n_pages ? -1 : p * t.page + (int)pos % t.page;
 }
 
@@ -345,12 +371,12 @@ kv_read_kernel(const Side k, const Side v, const Table t, int heads, const RowSh
       if (at[u] >= 0) {
         const size_t row = (size_t)at[u] * heads + head;
         if (MXF) {
-          const uint2 q = __ldg(reinterpret_cast<const uint2*>(sd.codes + row * (dim / 2) + d0 / 2));
+          const uint2 q = load_common(reinterpret_cast<const uint2*>(sd.codes + row * (dim / 2) + d0 / 2));
           code[u] = make_uint4(q.x, q.y, 0, 0);
-          scale[u] = mx::scale_value(__ldg(sd.scales + row * (dim / 32) + d0 / 32));
+          scale[u] = mx::scale_value(load_common(sd.scales + row * (dim / 32) + d0 / 32));
         } else {
-          code[u] = ld_stream_u4(sd.codes + row * dim + d0);
-          scale[u] = __ldg(reinterpret_cast<const float*>(sd.scales) + row);
+          code[u] = mx::load_once(sd.codes + row * dim + d0);
+          scale[u] = load_common(reinterpret_cast<const float*>(sd.scales) + row);
         }
       } else {
         code[u] = make_uint4(0, 0, 0, 0), scale[u] = 0.0f;

@@ -70,6 +70,14 @@ __device__ __forceinline__ void decode8(uint32_t codes, float (&v)[8]) {
   }
 }
 
+// Loads of data that a kernel before this one wrote, used once.  Plain loads, not the read-only (.nc) form: under
+// programmatic launch this kernel's life overlaps the writer's, and the read-only path promises nothing then.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // Sixteen consecutive values of a thread, kept as they were loaded; two threads hold a block.  `amax` is the
 // largest magnitude in a form that `merge` combines and `amax_bits` turns into a float32 bit pattern ordered
 // like the magnitudes, a NaN above infinity.
@@ -82,13 +90,14 @@ struct Chunk<float> {
     if (wide) {  // 32-byte aligned
 #pragma unroll
       for (int i = 0; i < 16; i += 8)
-        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
-                     : "l"(p + i));
+                     : "l"(p + i)
+                     : "memory");
     } else {
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const uint4 v = ld_stream_u4(p + i);
+        const uint4 v = load_once(p + i);
         w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
       }
     }
@@ -115,13 +124,14 @@ struct Chunk<__nv_bfloat16> {
   uint32_t w[8];
   __device__ __forceinline__ void load(const __nv_bfloat16* p, int wide) {
     if (wide) {
-      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                    : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-                   : "l"(p));
+                   : "l"(p)
+                   : "memory");
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        const uint4 v = ld_stream_u4(p + 2 * i);
+        const uint4 v = load_once(p + 2 * i);
         w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
       }
     }

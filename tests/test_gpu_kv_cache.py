@@ -215,6 +215,28 @@ def test_a_long_cache_passes_32_bits(fmt):
     assert np.array_equal(host(k), want) and np.array_equal(host(v), want)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "mxfp4"])
+def test_every_read_sees_the_write_before_it(fmt):
+    """Write, read, write, read, .. with nothing in between: launches that overlap, rows that share memory
+    sectors with rows read before they were written."""
+    heads, dim, n = 2, 32, 96
+    cache = Q.kv_cache_alloc(4, 32, heads, dim, fmt)
+    x = torch.randn(n, heads, dim, device="cuda")
+    slots = [torch.tensor([i], device="cuda") for i in range(n)]
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    rows = [x[i:i + 1] for i in range(n)]
+    outs = [(torch.empty(n, heads, dim, device="cuda"), torch.empty(n, heads, dim, device="cuda")) for _ in range(n)]
+    torch.cuda.synchronize()
+    for i in range(n):
+        Q.kv_cache_write(cache, rows[i], rows[i], slots[i])
+        Q.kv_cache_read(cache, table, cu, n, out=outs[i])
+    want = _decode(*_encode(host(x), fmt), fmt)
+    for i in range(n):
+        for got in outs[i]:
+            assert np.array_equal(host(got)[:i + 1], want[:i + 1]) and not host(got)[i + 1:].any()
+
+
 def test_module_and_a_decoder_step_captured_and_replayed():
     """Projection, cache write, read-back and attention over what was read, as a decoding loop runs them:
     eager steps, then the same step replayed from a CUDA graph with new tokens."""

@@ -272,6 +272,20 @@ def test_layer_state_dict_and_workflows():
     assert rel < 0.5
 
 
+@pytest.mark.parametrize("rows", [4, 40])
+def test_layers_one_after_the_other_see_each_other(rows):
+    """A chain of products whose buffers are used again: launches that overlap."""
+    ws = [Q.mx_quantize(torch.randn(256, 256, device="cuda") / 16) for _ in range(4)]
+    x = torch.randn(rows, 256, device="cuda")
+    y, want = x, x
+    for i in range(40):
+        y = Q.mx_linear(y, *ws[i % 4])
+    for i in range(40):
+        torch.cuda.synchronize()
+        want = Q.mx_matmul(*Q.mx_quantize(want), *ws[i % 4])
+    assert torch.isfinite(y).all() and torch.equal(y, want)
+
+
 def test_captured_and_replayed():
     x = torch.randn(48, 512, device="cuda")
     w = Q.mx_quantize(torch.randn(384, 512, device="cuda"))

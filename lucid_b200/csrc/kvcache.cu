@@ -70,7 +70,8 @@ struct FastDiv {
 // overwritten: a CTA enters its tokens' slots into a hash table in shared memory (the latest token of a slot
 // wins there) and looks the slots of all later tokens up in it.  The table is many times too large, so that a
 // slot which is not in it is nearly always told by one look.  (Inside the write itself the looks and their
-// barriers cost 5 of 22 us at 8192 tokens, and more than the rows at 32.)
+// barriers cost 5 of 22 us at 8192 tokens, and more than the rows at 32.  The comparison in the warp takes 4.9 us
+// for the whole write of 256 tokens, the two kernels 4.5, but one launch and one allocation less of the host's.)
 constexpr int kInline = 256;
 constexpr int kMarkThreads = 1024;
 template <int TOKENS>
@@ -331,7 +332,7 @@ __device__ __forceinline__ long long find_slot(const Table& t, long long r, bool
 // cu_seqlens and the page table is a chain of dependent loads, so it is walked for all rows at once), then
 // walk the rows' values together, 16 of a head per lane and step, four steps' loads in flight.  Bound by HBM:
 // a byte (half a byte) read and two or four written per value; 67615 rows of 8 x 128 to bf16: 71.5 us in int8 (5.9
-// TB/s), 69.7 in MXFP4.
+// TB/s), 69.9 in MXFP4.
 template <typename T, bool MXF, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
 kv_read_kernel(const Side k, const Side v, const Table t, int heads, const RowShape shape, long long total, int clear_tail,
@@ -435,8 +436,9 @@ int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bit
   int group_bits = MXF ? 1 : 0;
   while (group_bits < 5 && (16 << group_bits) < dim) ++group_bits;
   if (tokens > kInline) {
-    // few CTAs, each of which looks at the slots of all later tokens
-    if (int rc = tokens <= 16384 ? mark<128>(slots, slot_bits, tokens, dead, st) : mark<1024>(slots, slot_bits, tokens, dead, st)) return rc;
+    // every CTA looks at the slots of all later tokens: few tokens a CTA until the looks outweigh the shorter
+    // table (us of the whole write, 128 / 1024 tokens a CTA: 32768 tokens 46.1 / 49.1, 131072 212 / 184)
+    if (int rc = tokens <= 65536 ? mark<128>(slots, slot_bits, tokens, dead, st) : mark<1024>(slots, slot_bits, tokens, dead, st)) return rc;
   } else {
     dead = nullptr;
   }
@@ -507,27 +509,31 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   const RowShape shape = {2 * side_chunks, side_chunks, SmallDiv(head_chunks), 32 / (2 * side_chunks), 32 % (2 * side_chunks)};
   const int wide = ((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) % 32 == 0) &&
                    ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
-  // four rows a warp once that still gives every SM a few dozen warps; one row below
-  const bool few = total < 4 * 32 * (size_t)sm_count();
-  const size_t warps = few ? total : (total + 3) / 4;
+  // Rows a warp: one, or four or sixteen of short rows once that still leaves enough warps (their look-ups then
+  // overlap).  Measured, 1 / 4 / 16 rows, us: int8 67615 rows of 8 x 128 in 32 sequences 74.9 / 71.5, 16384 in one 19.6 /
+  // 22.3 / 32.8; 16384 rows of 8 x 64 13.5 / 10.5 / 17.1, 4096 4.7 / 5.2 / 13.7; 65536 rows of 1 x 64 37.7 / 11.5 / 6.3;
+  // MXFP4 65536 rows of 8 x 128 71.6 / 66.6 / 66.7.
+  auto fits = [&](size_t n) {
+    const size_t work = n * shape.chunks;  // chunks of sixteen values a warp
+    const size_t enough = work <= 128 ? 1024 : (work <= 256 || format == LQ_KV_MXFP4 ? 4096 : 16384);
+    return work <= 512 && total >= n * enough;
+  };
+  const size_t per_warp = fits(16) ? 16 : (fits(4) ? 4 : 1);
+  const size_t warps = (total + per_warp - 1) / per_warp;
   const unsigned grid = (unsigned)((warps * 32 + kThreads - 1) / kThreads);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
 #define LQ_KV_READ(T, F, N)                                                                                         \
   e = launch_pdl(kv_read_kernel<T, F, N>, dim3(grid), dim3(kThreads), 0, st, ks, vs, t, (int)heads, shape, (long long)total, \
                  clear_tail, wide, status)
-#define LQ_KV_READ_T(T)                                     \
-  if (format == LQ_KV_MXFP4) {                              \
-    if (few) LQ_KV_READ(T, true, 1);                        \
-    else LQ_KV_READ(T, true, 4);                            \
-  } else {                                                  \
-    if (few) LQ_KV_READ(T, false, 1);                       \
-    else LQ_KV_READ(T, false, 4);                           \
-  }
+#define LQ_KV_READ_T(T, F)                     \
+  if (per_warp == 1) LQ_KV_READ(T, F, 1);      \
+  else if (per_warp == 4) LQ_KV_READ(T, F, 4); \
+  else LQ_KV_READ(T, F, 16);
   if (out_dtype == LQ_F32) {
-    LQ_KV_READ_T(float)
+    if (format == LQ_KV_MXFP4) { LQ_KV_READ_T(float, true) } else { LQ_KV_READ_T(float, false) }
   } else {
-    LQ_KV_READ_T(bf16)
+    if (format == LQ_KV_MXFP4) { LQ_KV_READ_T(bf16, true) } else { LQ_KV_READ_T(bf16, false) }
   }
 #undef LQ_KV_READ_T
 #undef LQ_KV_READ

@@ -10,12 +10,14 @@ from ...quantization._kv_cache import KVCache, kv_cache_alloc, kv_cache_read, kv
 
 class PagedKVCache(torch.nn.Module):
     """``num_pages`` pages of ``page_size`` tokens, ``heads`` x ``head_dim`` values each for keys and for
-    values; ``fmt`` ``"int8"`` or ``"mxfp4"`` (:mod:`lucid_b200.quantization._kv_cache`)."""
+    values; ``fmt`` ``"int8"`` or ``"mxfp4"`` (:mod:`lucid_b200.quantization._kv_cache`).  Like the other
+    modules it is made on the CPU and moved by ``.cuda()``, or made where ``device`` says."""
 
     def __init__(self, num_pages: int, page_size: int, heads: int, head_dim: int, fmt: str = "int8", device=None) -> None:
         super().__init__()
         self.page_size, self.heads, self.head_dim, self.fmt = page_size, heads, head_dim, fmt
-        for name, t in kv_cache_alloc(num_pages, page_size, heads, head_dim, fmt, device)._asdict().items():
+        alloc = kv_cache_alloc(num_pages, page_size, heads, head_dim, fmt, "cpu" if device is None else device)
+        for name, t in alloc._asdict().items():
             self.register_buffer(name, t, persistent=False)
 
     @property

@@ -95,6 +95,8 @@ def test_cpu_tensors_and_shapes_are_refused():
         Q.kv_cache_write(Q.KVCache(*(torch.zeros(1, 1, 1, 16),) * 4), x, x, x)
     cache = Q.kv_cache_alloc(3, 4, 2, 64, "mxfp4", device="cpu")
     assert [tuple(t.shape) for t in cache] == [(3, 4, 2, 32), (3, 4, 2, 2)] * 2
+    module = nnq.PagedKVCache(3, 4, 2, 64)
+    assert list(module.state_dict()) == [] and module.cache.k_codes.shape == (3, 4, 2, 64) and not module.k_codes.is_cuda
     lin = nnq.MXLinear(288, 130)
     assert {k: tuple(v.shape) for k, v in lin.state_dict().items()} == {
         "weight_codes": (130, 144), "weight_scales": (2, 2, 1024), "bias": (130,)}

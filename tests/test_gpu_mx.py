@@ -266,10 +266,14 @@ def test_layer_state_dict_and_workflows():
     other = nnq.MXLinear(128, 256).cuda()
     other.load_state_dict(qmodel[0].state_dict())
     assert torch.equal(other(x), qmodel[0](x)) and "mxfp4" in repr(other)
-    # 4-bit operands: each element off by at most 1/6 of its block's top (steps of 2 below 6..8), the errors
-    # of a sum add up like a random walk; half the result's size is far outside that
-    rel = float((qmodel[0](x) - model[0](x)).norm() / model[0](x).norm())
-    assert rel < 0.5
+    # against the float layer: off by what rounding the operands moves, |x' - x| |w| + |x'| |w' - w|, and the sums'
+    # own rounding (130 additions each side)
+    xa, xb = x.double(), Q.mx_fake_quantize(x).double()
+    wa, wb = model[0].weight.detach().double(), Q.mx_fake_quantize(model[0].weight.detach()).double()
+    moved = (xb - xa).abs() @ wa.abs().T + xb.abs() @ (wb - wa).abs().T
+    with torch.no_grad(), _lib.ieee_float32():
+        apart = (qmodel[0](x).double() - model[0](x).double()).abs()
+    assert (apart <= moved + 2 * 130 * 2.0 ** -23 * size.double()).all() and float(apart.max()) > 0
 
 
 @pytest.mark.parametrize("rows", [4, 40])

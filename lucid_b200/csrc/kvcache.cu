@@ -213,10 +213,10 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 }
 
 // blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
-// (32 / group), all loads first; no warp waits for another.  8192 tokens of 8 x 128 bf16: 16.6 us in int8, 13.6 in
-// MXFP4 (3.1 TB/s), bound by instruction issue.  MARKED: the kernel before this one marks the
-// overwritten tokens.  It began after everything that wrote the rows was complete, so they are fetched while it
-// still runs, and only its marks are waited for.
+// (32 / group), all loads first; no warp waits for another.  8192 tokens of 8 x 128 bf16, with the marking: 18.7 us in
+// int8, 15.6 in MXFP4 (2.7 TB/s).  MARKED: the kernel before this one marks the overwritten tokens.  The rows, which
+// an earlier kernel wrote, are not fetched while that one runs (16.6 and 13.6 us): only griddepcontrol.wait promises
+// this grid the writes of the kernels before it.
 template <typename T, bool MXF, int CHUNKS, int ROWS, bool MARKED>
 __global__ void __launch_bounds__(kThreads)
 kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, uint32_t tokens, long long n_slots,
@@ -226,7 +226,8 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
   const Side& sd = blockIdx.y ? v : k;
   const int heads = (int)by_heads.d, across = 32 >> group_bits;
   const long long r0 = ((long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (ROWS * across) + (lane >> group_bits);
-  if (!MARKED) pdl_wait();
+  pdl_wait();
+  pdl_launch_dependents();
   Row<T, CHUNKS> x[ROWS];
   long long slot[ROWS];
   uint32_t token[ROWS];
@@ -240,8 +241,6 @@ kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int 
     x[u].load(reinterpret_cast<const T*>(sd.rows) + token[u] * sd.token + head[u] * sd.head, dim / 16, group, sub, ok, wide);
     slot[u] = ok ? index_at(slots, slot_bits, token[u]) : -1;
   }
-  if (MARKED) pdl_wait();
-  pdl_launch_dependents();
   if constexpr (MARKED) {
 #pragma unroll
     for (int u = 0; u < ROWS; ++u)

@@ -1,0 +1,49 @@
+"""Launches that overlap, each reading what the kernel right before it rewrote in place."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import lucid_b200.quantization as Q  # noqa: E402
+from lucid_b200 import _lib  # noqa: E402
+
+
+def _product_into(out, a, w):
+    """``out`` = a @ w.T by the library's own product, into memory that is used again and again."""
+    (ac, sa), (wc, sw) = a, w
+    m, n = out.shape
+    _lib.call("lq_mx_matmul", out.device, ac.data_ptr(), sa.data_ptr(), m, wc.data_ptr(), sw.data_ptr(), n, ac.shape[1] * 2, None,
+              0, out.data_ptr(), _lib.code_of(out.dtype), n, _lib.status_ptr(out.device))
+
+
+@pytest.mark.parametrize("tokens", [40, 300, 1500])
+@pytest.mark.parametrize("fmt", ["int8", "mxfp4"])
+def test_rows_and_slots_rewritten_before_each_write(fmt, tokens):
+    heads, dim, page, steps = 4, 64, 16, 12
+    pages = -(-tokens // page) + 2
+    a = [Q.mx_quantize(torch.randn(tokens, 256, device="cuda")) for _ in range(steps)]
+    w = [Q.mx_quantize(torch.randn(heads * dim, 256, device="cuda")) for _ in range(2)]
+    order = [torch.randperm(pages * page, device="cuda")[:tokens] for _ in range(steps)]
+    k, v = (torch.zeros(tokens, heads * dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.empty(tokens, dtype=torch.int64, device="cuda")
+    got, want = ([Q.kv_cache_alloc(pages, page, heads, dim, fmt) for _ in range(steps)] for _ in range(2))
+
+    def run(caches, between):
+        for i in range(steps):
+            slots.copy_(order[i])
+            between()
+            _product_into(k, a[i], w[0])
+            between()
+            _product_into(v, a[i], w[1])
+            between()
+            Q.kv_cache_write(caches[i], k.view(tokens, heads, dim), v.view(tokens, heads, dim), slots)
+            between()
+
+    torch.cuda.synchronize()
+    run(got, lambda: None)
+    torch.cuda.synchronize()
+    run(want, torch.cuda.synchronize)
+    for x, y in zip(got, want):
+        assert all(torch.equal(s, t) for s, t in zip(x, y)) and int(x.k_codes.view(torch.uint8).max()) > 0
+    _lib.check_device_status(k.device)

@@ -47,3 +47,28 @@ def test_rows_and_slots_rewritten_before_each_write(fmt, tokens):
     for x, y in zip(got, want):
         assert all(torch.equal(s, t) for s, t in zip(x, y)) and int(x.k_codes.view(torch.uint8).max()) > 0
     _lib.check_device_status(k.device)
+
+
+@pytest.mark.parametrize("rows,n", [(4, 200), (30, 300), (60, 300), (200, 4200), (700, 4200), (1300, 4100)])
+def test_weights_encoded_in_place_before_each_product(rows, n):
+    """Every form of the product: fused, one tile a CTA of 32, 64 and 128 tokens, CTA pairs."""
+    k, steps = 512, 8
+    src = [torch.randn(n, k, device="cuda") for _ in range(steps)]
+    x = [torch.randn(rows, k, device="cuda") for _ in range(steps)]
+    wc, sw = Q.mx_quantize(src[0])
+
+    def run(between):
+        ys = []
+        for i in range(steps):
+            _lib.call("lq_mx_quantize", wc.device, src[i].data_ptr(), _lib.code_of(torch.float32), n, k, k, wc.data_ptr(), sw.data_ptr())
+            between()
+            ys.append(Q.mx_linear(x[i], wc, sw))
+            between()
+        return ys
+
+    torch.cuda.synchronize()
+    got = run(lambda: None)
+    torch.cuda.synchronize()
+    want = run(torch.cuda.synchronize)
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
+    _lib.check_device_status(wc.device)

@@ -39,7 +39,7 @@ def test_the_scan_finds_the_kernels():
     assert set(OVERLAPPING) <= set(KERNELS)
 
 
-@pytest.mark.parametrize("name", OVERLAPPING)
+@pytest.mark.parametrize("name", OVERLAPPING + ["gemm_mx.cu:mx_tile_kernel"])
 def test_nothing_is_read_before_the_wait(name):
     before = KERNELS[name].split("pdl_wait();")[0]
     assert ACCESS.findall(before) == []

@@ -217,13 +217,14 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // Every warp waits here, the multiplying one too: a bounded wait on the first stage that began while the kernel
+  // before this one still ran would run out on that kernel's time.  The weight too is fetched only now: an earlier
+  // kernel may have encoded it, and the wait is what makes its writes visible here.  (48 x 8192 x 10240 15.3 us; 14.6
+  // with its first stages in flight during the encode of the activations.)
+  pdl_wait();
+  pdl_launch_dependents();
 
   if (warp == 0) {
-    // The weight too is fetched only now: an earlier kernel may have encoded it, and the wait is what makes its
-    // writes visible here.  (48 x 8192 x 10240 15.3 us; 14.6 with its first stages in flight during the encode of
-    // the activations.)
-    pdl_wait();
-    pdl_launch_dependents();
     int s = 0;
     uint32_t phase = 1;
     for (int i = 0; i < n; ++i) {
@@ -279,7 +280,6 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
   if constexpr (kFused) {
     static_assert(TN == 16, "one scale tile, two swizzle atoms of tokens");
     if (epilogue) {
-      pdl_wait();
       const int tid = (int)threadIdx.x - 64;
       // a thread encodes chunk c of sixteen values of row r and of row r + 8
       const int c = tid & 15, r = tid >> 4;
@@ -338,7 +338,6 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
     }
   }
   if (epilogue) {
-    if (!kFused) pdl_wait();
     ok = mbar_wait_warp(bar_done, 0, abort_flag, g.budget);
     tc_fence_after();
   }
@@ -369,7 +368,6 @@ mx_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__
         for (int j = 0; j < 16; ++j) part[(c + j) * kRows + quad * 32 + lane] = __uint_as_float(r[j]);
       }
     }
-    if (!epilogue) pdl_wait();
     cluster_sync_all();
     // four features a step; the loads from all CTAs are issued before the first addition
     const int total = valid * (kRows / 4);

@@ -1,5 +1,6 @@
 """The quantized key / value cache as a module: its tensors are buffers, so it moves with the model it
-belongs to (they are state of a run, not of a checkpoint, and stay out of ``state_dict``)."""
+belongs to, whose changes of type leave it alone (they are state of a run, not of a checkpoint, and stay out of
+``state_dict``)."""
 
 from __future__ import annotations
 
@@ -19,6 +20,15 @@ class PagedKVCache(torch.nn.Module):
         alloc = kv_cache_alloc(num_pages, page_size, heads, head_dim, fmt, "cpu" if device is None else device)
         for name, t in alloc._asdict().items():
             self.register_buffer(name, t, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        # ``model.to(torch.bfloat16)`` means the model's weights: the types of a cache are those of its format, and its
+        # float32 scales would lose bits on the way
+        def keep_type(t):
+            moved = fn(t)
+            return moved if moved.dtype == t.dtype else t.to(moved.device)
+
+        return super()._apply(keep_type, recurse)
 
     @property
     def cache(self) -> KVCache:

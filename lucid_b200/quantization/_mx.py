@@ -13,6 +13,7 @@ read (``rows`` being the product of the leading axes)."""
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from .. import _lib
 
@@ -104,19 +105,28 @@ def _pass_gradient(grad: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _has_tangent(t: torch.Tensor) -> bool:
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 class _StraightThrough(torch.autograd.Function):
     """The gradient of the fake quantization: linear in the gradient that comes in, so it is its own
-    derivative."""
+    derivative, forwards and backwards."""
 
     @staticmethod
     def forward(ctx, grad, mask):
         ctx.save_for_backward(mask)
+        ctx.save_for_forward(mask)
         return _pass_gradient(grad, mask)
 
     @staticmethod
     def backward(ctx, grad):
         (mask,) = ctx.saved_tensors
         return _StraightThrough.apply(grad, mask), None
+
+    @staticmethod
+    def jvp(ctx, tangent, _):
+        return _StraightThrough.apply(tangent, *ctx.saved_tensors)
 
 
 def _fake_quantize(x: torch.Tensor, want_mask: bool):
@@ -132,22 +142,27 @@ class _MXFakeQuantize(torch.autograd.Function):
     def forward(ctx, x):
         out, mask = _fake_quantize(x, True)
         ctx.save_for_backward(mask)
+        ctx.save_for_forward(mask)
         return out
 
     @staticmethod
     def backward(ctx, grad):
         (mask,) = ctx.saved_tensors
-        if torch.is_grad_enabled():  # create_graph: somebody differentiates the gradient
+        if torch.is_grad_enabled() or _has_tangent(grad):  # somebody differentiates the gradient
             return _StraightThrough.apply(grad, mask)
         return _pass_gradient(grad, mask)
+
+    @staticmethod
+    def jvp(ctx, tangent):
+        return _StraightThrough.apply(tangent, *ctx.saved_tensors)
 
 
 def mx_fake_quantize(x: torch.Tensor) -> torch.Tensor:
     """``mx_dequantize(*mx_quantize(x))`` in one pass, in ``x``'s dtype, with the straight-through
     gradient: it passes where the element was rounded inside the grid and is zero where it was clamped
-    (and in blocks that decode to NaN).  A backward pass is captured in a CUDA graph as any of torch's:
-    with no eager graph of the same leaves alive on another stream."""
-    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+    (and in blocks that decode to NaN); a forward-mode tangent passes likewise.  A backward pass is captured in a
+    CUDA graph as any of torch's: with no eager graph of the same leaves alive on another stream."""
+    if isinstance(x, torch.Tensor) and (x.requires_grad and torch.is_grad_enabled() or _has_tangent(x)):
         return _MXFakeQuantize.apply(x)
     return _fake_quantize(x, False)[0]
 

@@ -508,7 +508,8 @@ int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_
  *                lq_quantize_per_token on the grid [-128, 127] with eps 1e-8, a (token, head) being a row;
  *                a row that holds a NaN or an infinity takes a NaN scale.  dim % 16 == 0.
  *   LQ_KV_MXFP4: codes (.., dim / 2) and scale bytes (.., dim / 32) in block order.  dim % 32 == 0.
- * dim <= 1024.  No counterpart in the reference. */
+ * dim <= 1024, heads <= 4096.  The tensors of a cache without pages, and a table without entries, may be NULL.  No
+ * counterpart in the reference. */
 enum lq_kv_format { LQ_KV_INT8 = 0, LQ_KV_MXFP4 = 1 };
 
 /* Encode k and v, (tokens, heads, dim) with element strides (token, head) and contiguous dim, LQ_F32 |

@@ -457,7 +457,9 @@ extern "C" int lq_kv_write(const void* k, const void* v, int in_dtype, size_t to
                            void* k_codes, void* k_scales, void* v_codes, void* v_scales, void* workspace, size_t workspace_bytes,
                            int32_t* status, void* stream) {
   if (tokens == 0) return LQ_OK;
-  if (!k || !v || !slots || !k_codes || !k_scales || !v_codes || !v_scales) return fail(LQ_ERR_DEVICE, "lq_kv_write: null pointer");
+  // a cache without pages has no memory: every slot is past it
+  if (!k || !v || !slots || (n_slots > 0 && (!k_codes || !k_scales || !v_codes || !v_scales)))
+    return fail(LQ_ERR_DEVICE, "lq_kv_write: null pointer");
   if (in_dtype != LQ_F32 && in_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_kv_write: k and v must be f32|bf16");
   if (slot_bits != 32 && slot_bits != 64) return fail(LQ_ERR_DTYPE, "lq_kv_write: slots must be int32 or int64");
   if (int rc = check_format("lq_kv_write", format, heads, dim)) return rc;
@@ -489,7 +491,8 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
                           void* out_k, void* out_v, int out_dtype, size_t k_token, size_t k_head, size_t v_token, size_t v_head,
                           int clear_tail, int32_t* status, void* stream) {
   if (total == 0) return LQ_OK;
-  if (!k_codes || !k_scales || !v_codes || !v_scales || !out_k || !out_v || !cu_seqlens || (!table && max_blocks > 0))
+  if (!out_k || !out_v || !cu_seqlens || (!table && seqs > 0 && max_blocks > 0) ||
+      (n_pages > 0 && (!k_codes || !k_scales || !v_codes || !v_scales)))
     return fail(LQ_ERR_DEVICE, "lq_kv_read: null pointer");
   if (out_dtype != LQ_F32 && out_dtype != LQ_BF16) return fail(LQ_ERR_DTYPE, "lq_kv_read: out must be f32|bf16");
   if (int rc = check_format("lq_kv_read", format, heads, dim)) return rc;

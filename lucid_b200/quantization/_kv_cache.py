@@ -26,13 +26,14 @@ class KVCache(NamedTuple):
 
 
 def kv_cache_alloc(num_pages: int, page_size: int, heads: int, head_dim: int, fmt: str = "int8", device=None) -> KVCache:
-    """A cache of zeros; ``fmt`` is ``"int8"`` (head_dim a multiple of 16) or ``"mxfp4"`` (of 32)."""
+    """A cache of zeros; ``fmt`` is ``"int8"`` (head_dim a multiple of 16) or ``"mxfp4"`` (of 32); up to 4096
+    heads of up to 1024 values.  A cache without pages is one that every slot and every page lies outside."""
     if fmt not in _FORMATS:
         raise ValueError(f"cache format must be one of {sorted(_FORMATS)}, got {fmt!r}")
     step = 16 if fmt == "int8" else 32
     if head_dim <= 0 or head_dim % step or head_dim > 1024:
         raise _lib.ShapeMismatch(f"head_dim must be a multiple of {step} up to 1024 for {fmt}, got {head_dim}")
-    if num_pages < 0 or page_size <= 0 or heads <= 0:
+    if num_pages < 0 or page_size <= 0 or heads <= 0 or heads > 4096:
         raise _lib.ShapeMismatch(f"{num_pages} pages of {page_size} tokens x {heads} heads")
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     lead = (num_pages, page_size, heads)

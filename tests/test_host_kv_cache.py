@@ -34,3 +34,10 @@ def test_the_cache_still_moves_between_devices():
     assert all(t.is_meta and t.dtype == d for t, d in zip(module.cache, types))
     module.to_empty(device="cpu")
     assert all(not t.is_meta and t.dtype == d for t, d in zip(module.cache, types))
+
+
+def test_a_cache_that_no_call_would_take_is_not_made():
+    for heads in (0, 4097):
+        with pytest.raises(_lib.ShapeMismatch):
+            Q.kv_cache_alloc(1, 1, heads, 32, device="cpu")
+    assert Q.kv_cache_alloc(1, 1, 4096, 32, device="cpu").k_scales.shape == (1, 1, 4096)

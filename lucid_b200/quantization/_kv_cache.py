@@ -87,6 +87,21 @@ def _distinct_rows(t: torch.Tensor) -> bool:
            ((n <= 1 or sn >= d) and (h <= 1 or sh >= (n - 1) * sn + d))
 
 
+def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two ``(tokens, heads, dim)`` tensors, each of distinct rows, share an address.  Answered for
+    equal strides (halves of one buffer, however they interleave) and equal beginnings."""
+    if a.numel() == 0:
+        return False
+    apart = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
+    (n, h, d), (sn, sh, _) = a.shape, a.stride()
+    if apart and (a.stride() != b.stride() or apart >= (n - 1) * sn + (h - 1) * sh + d):
+        return False
+    left = [apart]  # what is left of the distance after whole steps of the longer stride, then of the shorter
+    for step, count in sorted(((s, c) for s, c in ((sn, n), (sh, h)) if c > 1), reverse=True):
+        left = [r - i * step for r in left for i in (r // step, r // step + 1) if -count < i < count]
+    return any(-d < r < d for r in left)
+
+
 def kv_cache_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Encode the new rows ``k``, ``v`` ``(tokens, heads, dim)`` (float32 or bfloat16; strided views such as
     slices of a fused projection are read in place) into ``slots`` ``(tokens,)`` (int32 or int64).
@@ -131,8 +146,8 @@ def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.
     ``cu_seqlens`` int32 ``(sequences + 1,)`` says which output rows belong to which sequence, and row
     ``cu_seqlens[b] + i`` is its token ``starts[b] + i`` (``starts`` int32, default zeros).  ``total`` is the
     number of output rows, known to the host.  ``out=(k, v)`` writes into given float32 / bfloat16
-    tensors of any token and head stride; rows that no sequence covers keep what they held there,
-    and are zeros in tensors allocated here.  A token past its row of the table, or a page outside
+    tensors of any token and head stride, no two rows of which overlap; rows that no sequence covers keep
+    what they held there, and are zeros in tensors allocated here.  A token past its row of the table, or a page outside
     the cache, reads as zeros and sets the device status word."""
     fmt, pages, page, heads, dim, dev = _check_cache(cache)
     _lib.require_cuda(block_tables, "block_tables")
@@ -175,6 +190,8 @@ def kv_cache_read(cache: KVCache, block_tables: torch.Tensor, cu_seqlens: torch.
                 raise _lib.ShapeMismatch(f"out= is {tuple(t.shape)}, expected {shape}")
             if not _row_view(t) or not _distinct_rows(t):
                 raise _lib.ShapeMismatch("out= needs a contiguous last axis and 16-byte aligned rows that do not overlap")
+        if _rows_meet(ok, ov):
+            raise _lib.ShapeMismatch("out= has keys and values in the same memory")
     table = block_tables if max_blocks <= 1 or block_tables.stride(1) == 1 else block_tables.contiguous()
     cu = cu_seqlens.contiguous()
     kt, kh, _ = ok.stride()

@@ -477,7 +477,8 @@ size_t lq_mx_scale_bytes(size_t rows, size_t K);
  * scale tiles is written as 0. */
 int lq_mx_quantize(const void* x, int in_dtype, size_t rows, size_t K, size_t ldx, uint8_t* codes,
                    uint8_t* scales, void* stream);
-/* out: (rows, K) contiguous, LQ_F32 | LQ_BF16 (both hold every finite value of the format exactly). */
+/* out: (rows, K) contiguous, LQ_F32 | LQ_BF16.  Both hold exactly whatever lq_mx_quantize encodes.  With the scale bytes
+ * 253 and 254, which it never writes (its largest is 252), products from 2^128 on become infinities. */
 int lq_mx_dequantize(const uint8_t* codes, const uint8_t* scales, size_t rows, size_t K, void* out,
                      int out_dtype, void* stream);
 /* out = decode(encode(x)) over n contiguous values (n a multiple of 32), out of x's dtype.  mask

@@ -87,7 +87,8 @@ def mx_quantize(x: torch.Tensor):
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The values ``(codes, scales)`` stand for: exact in float32 and in bfloat16."""
+    """The values ``(codes, scales)`` stand for: exact in float32 and in bfloat16, up to the float32 range (which a
+    scale byte of 253 or 254 can pass; ``mx_quantize`` writes none above 252)."""
     if out_dtype not in _FLOATS:
         raise _lib.DtypeMismatch(f"mx_dequantize writes float32 or bfloat16, got {out_dtype}")
     c, s, rows, k = _check_packed(codes, scales, "mx_dequantize")

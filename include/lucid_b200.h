@@ -489,11 +489,13 @@ int lq_mx_fake_quantize(const void* x, int dtype, size_t n, void* out, uint8_t* 
 int lq_mx_fake_quantize_grad(const void* grad, int dtype, const uint8_t* mask, size_t n, void* out,
                              void* stream);
 /* out (M, N) = a (M, K) * w (N, K)^T (+ bias[N], float32) (ReLU), float32 accumulation; out LQ_F32 |
- * LQ_BF16, row stride ldo elements.  status: as for lq_gemm_s8. */
+ * LQ_BF16, row stride ldo elements.  status: as for lq_gemm_s8.  Whole tiles are multiplied: where K is no multiple of
+ * 256, the scale bytes past K must not be 255 (NaN times the zero codes there is NaN; lq_mx_quantize writes 0).  The
+ * scale bytes of rows past the end may be anything. */
 int lq_mx_matmul(const uint8_t* a_codes, const uint8_t* a_scales, size_t M, const uint8_t* w_codes,
                  const uint8_t* w_scales, size_t N, size_t K, const float* bias, int relu, void* out,
                  int out_dtype, size_t ldo, int32_t* status, void* stream);
-/* lq_mx_quantize of x into the workspace, then lq_mx_matmul; up to 16 rows in one launch without a
+/* lq_mx_quantize of x into the workspace, then lq_mx_matmul (which see for w_scales); up to 16 rows in one launch without a
  * workspace. */
 size_t lq_mx_linear_workspace_bytes(size_t M, size_t K);
 int lq_mx_linear(const void* x, int in_dtype, size_t M, size_t ldx, const uint8_t* w_codes,

@@ -8,7 +8,8 @@ weights and activations are encoded by the same call, activations on every forwa
 
 ``mx_quantize`` returns ``(codes, scales)``: ``codes`` is uint8 ``(..., K / 2)``, two elements a byte, and
 ``scales`` uint8 ``(ceil(rows / 128), ceil(K / 256), 1024)``, the scale bytes in the tiles the tensor cores
-read (``rows`` being the product of the leading axes)."""
+read (``rows`` being the product of the leading axes).  ``mx_quantize`` fills the tiles' padding with 0; tiles
+made elsewhere may hold anything there but 255 (NaN) past ``K``, which a product multiplies with zeros."""
 
 from __future__ import annotations
 

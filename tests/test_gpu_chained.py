@@ -72,3 +72,47 @@ def test_weights_encoded_in_place_before_each_product(rows, n):
     want = run(torch.cuda.synchronize)
     assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, want))
     _lib.check_device_status(wc.device)
+
+
+@pytest.mark.parametrize("tokens", [20, 700])
+@pytest.mark.parametrize("fmt", ["int8", "mxfp4"])
+def test_two_captured_steps_replayed_in_turn(fmt, tokens):
+    """Two graphs of write and read, each with workspaces of its own, replayed alternately with new rows, and an
+    eager step on another stream in between."""
+    heads, dim, page = 2, 64, 16
+    pages = -(-tokens // page)
+    caches = [Q.kv_cache_alloc(pages, page, heads, dim, fmt) for _ in range(3)]
+    rows = [torch.zeros(tokens, heads, dim, device="cuda") for _ in range(3)]
+    slots = [torch.randint(-2, pages * page, (tokens,), device="cuda") for _ in range(3)]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, pages * page], dtype=torch.int32, device="cuda")
+
+    def step(i):
+        Q.kv_cache_write(caches[i], rows[i], -rows[i], slots[i])
+        return Q.kv_cache_read(caches[i], table, cu, pages * page, out_dtype=torch.bfloat16)
+
+    step(0)
+    graphs, outs = [], []
+    for i in range(2):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(step(i))
+    side = torch.cuda.Stream()
+    for turn in range(4):
+        for i in range(3):
+            rows[i].copy_(torch.randn(tokens, heads, dim, device="cuda"))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step(2)
+        for i in (0, 1, 0):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in (*outs, other)]
+        for i in range(3):
+            for t in caches[i]:
+                t.zero_()
+            want = step(i)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) and b.any() for a, b in zip(got[i], want)), (turn, i)
+    _lib.check_device_status(cu.device)

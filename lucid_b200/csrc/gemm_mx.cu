@@ -158,8 +158,10 @@ __device__ __forceinline__ void store_block(const Args& g, const float (&y)[COUN
 // a cluster each take a contiguous run of K, so that a narrow layer still occupies the GPU, and two CTAs
 // fit an SM, so that the copies of one run during the epilogue of the other.  The partial sums meet in
 // shared memory: every CTA reads the others' through the cluster and adds them in rank order (the same
-// result whatever the timing), each for its share of the outputs.  1 x 8192 x 28672: 23.2 us, 5.4 TB/s of weight;
-// below that, launch, fill and exchange add about 4 us to the stream.
+// result whatever the timing), each for its share of the outputs.  1 x 8192 x 28672: 21.3 us, 5.9 TB/s of weight;
+// below that, launch, fill and exchange add about 4 us to the stream.  1000 x 4096 x 4096 to float32 (128 tokens a tile,
+// one wave of 256 CTAs): 14.3 us with the tensor cores 29 % and L2 25 % busy; neither bounds it, the time is the fill of
+// the ring, 16 stages, and an epilogue that little overlaps.
 constexpr int kMaxSplit = 8;
 constexpr int kThreads = 192;  // producer, multiply, four epilogue warps
 
@@ -638,8 +640,8 @@ struct Operands {
   size_t M, N, K;
 };
 // Up to this many rows lq_mx_linear encodes them inside the product.  More take longer to encode in every CTA than
-// in a kernel of their own: 32 x 8192 x 8192 15.2 us against 11.9, 48 x 8192 x 10240 23.5 against 14.5; at 16 x 8192 x
-// 28672 24.7 against 23.9, and one launch of the host's time less.
+// in a kernel of their own: 32 x 8192 x 8192 15.2 us against 12.7, 48 x 8192 x 10240 23.5 against 14.6; at 16 x 8192 x
+// 28672 24.2 against 24.3, 8 x 8192 x 8192 9.2 against 11.4, and one launch of the host's time less.
 constexpr size_t kFusedTokens = 16;
 
 template <int TN, typename T, typename X = void>

@@ -1,7 +1,7 @@
 // The quantized key / value cache: rows encoded as they are written, and read back by page table.
 //
 // A cache row is one token's (heads, dim) values, kept contiguous (page, offset, head, dim), so a write is one
-// pass over the new tokens and a read one pass over the tokens asked for; both are bound by HBM.  Two formats:
+// pass over the new tokens and a read one pass over the tokens asked for.  Two formats:
 // int8 codes with one float32 scale per (token, head) -- the arithmetic of the per-token encode -- and
 // MXFP4 along the head dimension.
 #include <cuda_fp16.h>
@@ -69,9 +69,11 @@ struct FastDiv {
 // its slot with those of all later tokens itself; for more, a kernel of its own marks the tokens that are
 // overwritten: a CTA enters its tokens' slots into a hash table in shared memory (the latest token of a slot
 // wins there) and looks the slots of all later tokens up in it.  The table is many times too large, so that a
-// slot which is not in it is nearly always told by one look.  (Inside the write itself the looks and their
-// barriers cost 5 of 22 us at 8192 tokens, and more than the rows at 32.  The comparison in the warp takes 4.9 us
-// for the whole write of 256 tokens, the two kernels 4.5, but one launch and one allocation less of the host's.)
+// slot which is not in it is nearly always told by one look.  The looks grow with the square of the tokens, and with
+// narrow rows they are most of the time: 1 x 64 in MXFP4, 8192 tokens 7.8 us, 131072 62 us (6.5 us of rows at the
+// measured copy's rate).  (Inside the write itself the looks and their barriers cost 5 of 22 us at 8192 tokens, and
+// more than the rows at 32.  256 tokens of 8 x 128, the whole write: 5.0 us in int8 and 4.1 in MXFP4 with the comparison
+// in the warp, 5.3 and 4.4 with two kernels, which cost the host a launch and an allocation more.)
 constexpr int kInline = 256;
 constexpr int kMarkThreads = 1024;
 template <int TOKENS>
@@ -214,7 +216,7 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 
 // blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
 // (32 / group), all loads first; no warp waits for another.  8192 tokens of 8 x 128 bf16, with the marking: 18.7 us in
-// int8, 15.6 in MXFP4 (2.7 TB/s).  MARKED: the kernel before this one marks the overwritten tokens.  The rows, which
+// int8, 15.6 in MXFP4 (2.7 TB/s): the marking before it, then instruction issue (62 and 58 % of the cycles).  MARKED: the kernel before this one marks the overwritten tokens.  The rows, which
 // an earlier kernel wrote, are not fetched while that one runs (16.6 and 13.6 us): only griddepcontrol.wait promises
 // this grid the writes of the kernels before it.
 template <typename T, bool MXF, int CHUNKS, int ROWS, bool MARKED>
@@ -330,8 +332,8 @@ __device__ __forceinline__ long long find_slot(const Table& t, long long r, bool
 // A warp reads TOKENS consecutive output rows.  Its lanes first look up one row each (the search through
 // cu_seqlens and the page table is a chain of dependent loads, so it is walked for all rows at once), then
 // walk the rows' values together, 16 of a head per lane and step, four steps' loads in flight.  Bound by HBM:
-// a byte (half a byte) read and two or four written per value; 67615 rows of 8 x 128 to bf16: 71.5 us in int8 (5.9
-// TB/s), 69.9 in MXFP4.
+// a byte (half a byte) read and two or four written per value; 67615 rows of 8 x 128 to bf16: 72 us in int8 (5.8
+// TB/s), 70 in MXFP4.
 template <typename T, bool MXF, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
 kv_read_kernel(const Side k, const Side v, const Table t, int heads, const RowShape shape, long long total, int clear_tail,
@@ -436,7 +438,7 @@ int write_dispatch(const Side& k, const Side& v, const void* slots, int slot_bit
   while (group_bits < 5 && (16 << group_bits) < dim) ++group_bits;
   if (tokens > kInline) {
     // every CTA looks at the slots of all later tokens: few tokens a CTA until the looks outweigh the shorter
-    // table (us of the whole write, 128 / 1024 tokens a CTA: 32768 tokens 46.1 / 49.1, 131072 212 / 184)
+    // table (us of the whole write in MXFP4, 128 / 1024 tokens a CTA: 32768 tokens 45.8 / 49.3, 131072 213 / 175)
     if (int rc = tokens <= 65536 ? mark<128>(slots, slot_bits, tokens, dead, st) : mark<1024>(slots, slot_bits, tokens, dead, st)) return rc;
   } else {
     dead = nullptr;
@@ -512,9 +514,11 @@ extern "C" int lq_kv_read(const void* k_codes, const void* k_scales, const void*
   const int wide = ((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) % 32 == 0) &&
                    ((k_token | k_head | v_token | v_head) * esz) % 32 == 0;
   // Rows a warp: one, or four or sixteen of short rows once that still leaves enough warps (their look-ups then
-  // overlap).  Measured, 1 / 4 / 16 rows, us: int8 67615 rows of 8 x 128 in 32 sequences 74.9 / 71.5, 16384 in one 19.6 /
-  // 22.3 / 32.8; 16384 rows of 8 x 64 13.5 / 10.5 / 17.1, 4096 4.7 / 5.2 / 13.7; 65536 rows of 1 x 64 37.7 / 11.5 / 6.3;
-  // MXFP4 65536 rows of 8 x 128 71.6 / 66.6 / 66.7.
+  // overlap).  Measured, 1 / 4 / 16 rows, us, in one sequence (in 32): int8 8 x 128, 16384 rows 19.8 / 22.2 / 32.8 (20.9 /
+  // 22.9 / 33.3), 32768 35.9 / 37.1 / 42.9 (37.7 / 37.6 / 43.4), 49152 51.7 / 52.7 / 60.7 (54.0 / 53.7 / 60.3), 65536 67.9 /
+  // 68.1 / 80.0 (70.6 / 69.2 / 81.7); int8 8 x 64, 4096 4.7 / 5.1 / 13.6, 16384 13.5 / 10.4 / 17.1; int8 1 x 64, 4096 4.1 /
+  // 2.9 / 3.6, 16384 10.6 / 4.1 / 3.7, 65536 37.7 / 11.4 / 6.3; MXFP4 8 x 128, 16384 21.2 / 20.0 / 40.7, 65536 71.6 / 66.5 /
+  // 66.4; MXFP4 4 x 64, 4096 4.0 / 3.8 / 7.8, 36903 23.5 / 12.2 / 12.7, 65536 40.8 / 21.1 / 18.7.
   auto fits = [&](size_t n) {
     const size_t work = n * shape.chunks;  // chunks of sixteen values a warp
     const size_t enough = work <= 128 ? 1024 : (work <= 256 || format == LQ_KV_MXFP4 ? 4096 : 16384);

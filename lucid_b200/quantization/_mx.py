@@ -206,7 +206,8 @@ def mx_matmul(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tens
 
 def mx_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, bias: torch.Tensor | None = None,
               relu: bool = False) -> torch.Tensor:
-    """``mx_matmul(*mx_quantize(x), ...)`` in one call; the result has ``x``'s dtype."""
+    """``mx_matmul(*mx_quantize(x), ...)`` in one call; the result has ``x``'s dtype.  For inference, like the other
+    quantized products: no derivative passes (training goes through ``mx_fake_quantize``)."""
     x = _float_input(x, "mx_linear input")
     wc, sw, n, k = _check_packed(w_codes, w_scales, "mx_linear weight")
     if w_codes.dim() != 2:

@@ -216,9 +216,9 @@ __device__ __forceinline__ void encode_row(const Side& sd, const Row<T, CHUNKS>&
 
 // blockIdx.y: keys or values.  A warp takes ROWS times as many consecutive (token, head) rows as fit side by side
 // (32 / group), all loads first; no warp waits for another.  8192 tokens of 8 x 128 bf16, with the marking: 18.7 us in
-// int8, 15.6 in MXFP4 (2.7 TB/s): the marking before it, then instruction issue (62 and 58 % of the cycles).  MARKED: the kernel before this one marks the overwritten tokens.  The rows, which
-// an earlier kernel wrote, are not fetched while that one runs (16.6 and 13.6 us): only griddepcontrol.wait promises
-// this grid the writes of the kernels before it.
+// int8, 15.6 in MXFP4 (2.7 TB/s): the marking before it, then instruction issue (62 and 58 % of the cycles).  MARKED: the
+// kernel before this one marks the overwritten tokens.  The rows, which an earlier kernel wrote, are not fetched while
+// that one runs (16.6 and 13.6 us): only griddepcontrol.wait promises this grid the writes of the kernels before it.
 template <typename T, bool MXF, int CHUNKS, int ROWS, bool MARKED>
 __global__ void __launch_bounds__(kThreads)
 kv_write_kernel(const Side k, const Side v, const void* __restrict__ slots, int slot_bits, uint32_t tokens, long long n_slots,

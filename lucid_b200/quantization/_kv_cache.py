@@ -93,11 +93,12 @@ def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     if a.numel() == 0:
         return False
     apart = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
-    (n, h, d), (sn, sh, _) = a.shape, a.stride()
-    if apart and (a.stride() != b.stride() or apart >= (n - 1) * sn + (h - 1) * sh + d):
+    d = a.shape[2]
+    steps, others = (sorted(((s, c) for s, c in zip(t.stride()[:2], t.shape) if c > 1), reverse=True) for t in (a, b))
+    if apart and (steps != others or apart >= sum(s * (c - 1) for s, c in steps) + d):
         return False
     left = [apart]  # what is left of the distance after whole steps of the longer stride, then of the shorter
-    for step, count in sorted(((s, c) for s, c in ((sn, n), (sh, h)) if c > 1), reverse=True):
+    for step, count in steps:
         left = [r - i * step for r in left for i in (r // step, r // step + 1) if -count < i < count]
     return any(-d < r < d for r in left)
 

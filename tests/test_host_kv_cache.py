@@ -58,6 +58,7 @@ def _pairs(buf):
     yield buf.as_strided((5, 4, 32), (256, 32, 1), 16), buf.as_strided((5, 4, 32), (256, 32, 1), 144), False
     yield whole[0], buf.as_strided((6, 4, 32), (256, 32, 1)), True        # another stride from the same beginning
     yield whole[0, :1, :1], whole[0, :1, 1:2], False
+    yield whole[0, :1], buf.as_strided((1, 4, 32), (999, 32, 1), 16), True  # (the stride of a single token says nothing)
     yield whole[0, :0], whole[0, :0], False
 
 
